@@ -151,6 +151,56 @@ int k44b_plan_add_argmax(void *plan, const char *name, uint64_t src_off, uint32_
 int k44b_plan_set_tokens(void *plan, const int32_t *h_tokens, uint32_t n, void *stream);
 int k44b_plan_get_next_tokens(void *plan, int32_t *h_tokens, uint32_t n, void *stream);
 
+/* ---- decoder operators (no counterpart in the reference) ----
+ * Prompt attention with a sliding window and sinks: like add_rope_attn (blocks of seq_len columns, grouped-query heads, head_dim 64
+ * or 128), but seq_len may be any length, and column t of a sequence that starts at s0 sees column c if s0 <= c <= t and (window == 0,
+ * or c > t - window, or c < s0 + sinks). q and k are rotated on the way and stay as they are on the canvas; out must not overlap
+ * them. Prompts of different lengths are padded behind their last token. A hidden column does not count, whatever it holds. */
+int k44b_plan_add_window_attn(void *plan, const char *name, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off, uint32_t h_q,
+                              uint32_t h_kv, uint32_t head_dim, uint32_t seq_len, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling);
+/* Key / value cache of 8 bits. It lives in device memory of the caller (so that a prompt plan can fill it and a decode plan read it)
+ * and must outlive the plans that name it: k44b_kv8_bytes bytes on a 256-byte boundary, cleared once with k44b_kv8_clear. `columns`
+ * sequences of up to max_seq positions, h_kv heads of 64 or 128 dimensions. Per column, head and block of 64 positions there are
+ * e4m3 codes with one FP32 scale for the keys and one for the values, scale = max(amax, 2^-24) / 448, value = code * scale; the block
+ * that is still open is kept as FP16 rows. The parts, each starting on a multiple of 256 bytes:
+ *   codes      [column][head][block][ keys: head_dim / 64 | 64 positions | 64 dims ][ values: head_dim | 64 positions ]
+ *   scales     [column][head][block][keys, values] FP32
+ *   k_tail     [column][head][64 positions][head_dim] FP16       v_tail  [column][head][head_dim][64 positions] FP16
+ *   tail_block [column][head] int32, number of the open block, -1 none
+ * Infinities count as +-65504; a NaN stays a NaN of its own value. k44b_kv8_bytes returns 0 for impossible sizes. */
+typedef struct k44b_kv8_cache {
+    void *data;
+    uint64_t bytes;
+    uint32_t columns, h_kv, head_dim, max_seq;
+} k44b_kv8_cache;
+uint64_t k44b_kv8_bytes(uint32_t columns, uint32_t h_kv, uint32_t head_dim, uint32_t max_seq);
+int k44b_kv8_clear(const k44b_kv8_cache *cache, void *stream);
+/* Prompt into the cache: the keys (not yet rotated; they are rotated at positions 0, 1, ... of their sequence) and values of a prompt
+ * plan. set_sequences says, for the first n blocks of seq_len columns, which cache column a sequence goes to (-1: nowhere; no column
+ * twice) and how long it is; blocks from n on go nowhere. What the column held before is replaced; positions from the length on are
+ * left as they were. */
+int k44b_plan_add_kv8_fill(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t k_off, uint64_t v_off, uint32_t seq_len, float rope_theta,
+                           int llama3_scaling);
+int k44b_plan_set_sequences(void *plan, const int32_t *h_cache_columns, const int32_t *h_lengths, uint32_t n, void *stream);
+/* Decode attention against such a cache: plan column b is cache column b and holds one new token at its own position
+ * (set_positions: the first n columns, -1 = idle, the initial state of all; an advancing arg-max moves the positions of the columns
+ * that are not idle on by one). q and k are rotated at that position and stay as they are on the canvas, k and v are appended, and
+ * the column attends to positions 0 .. position under the same window and sinks as above. An idle column gets zeros and its cache is
+ * left alone. h_q / h_kv up to 16, at most 4096 columns. A position may go back: the positions behind it are given up, and those of its
+ * block keep their 8-bit values where the block was complete. A position outside the cache leaves its column idle and sets status
+ * bit 4. One execution of a plan at a time, and one plan at a time on a cache. */
+int k44b_plan_add_kv8_attn(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off,
+                           uint32_t h_q, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling);
+int k44b_plan_set_positions(void *plan, const int32_t *h_positions, uint32_t n, void *stream);
+/* Probabilities of an answer, per column of a logits tensor of `rows` channels, into device arrays of the caller: the natural logarithm of
+ * the probability of row targets[column] (NaN for a target that is no row), the entropy in nats, and the `top` (0 .. 32) most
+ * probable rows with their log probabilities, [top][columns], the lowest row first among equals. Logits of -infinity have
+ * probability 0; a column that holds a NaN or +infinity, or nothing above -infinity, has NaN probabilities. targets and logprobs may be
+ * null together, entropy alone, and the two arrays of alternatives with top = 0. */
+int k44b_plan_add_logprobs(void *plan, const char *name, uint64_t src_off, uint32_t rows, const int32_t *d_targets, float *d_logprobs, float *d_entropy,
+                           uint32_t top, int32_t *d_top_rows, float *d_top_logprobs);
+uint32_t k44b_plan_columns(void *plan);
+
 /* ---- neuron sharding over the GPUs of one box (no counterpart in the reference, which is single-GPU) ----
  * Every rank holds a plan with its rows of every wave and a full-size canvas. After k44b_plan_set_peers_* the wave
  * kernels store each output row into the rank's own canvas and into the peers' canvases (peer-mapped memory over

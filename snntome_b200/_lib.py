@@ -28,6 +28,11 @@ class PlaneGeom(ctypes.Structure):
     _fields_ = [("h", c_uint32), ("w", c_uint32), ("w_pad", c_uint32), ("plane_stride", c_uint32)]
 
 
+class KV8CacheDesc(ctypes.Structure):
+    """k44b_kv8_cache (include/k44b.h)."""
+    _fields_ = [("data", c_void_p), ("bytes", c_uint64), ("columns", c_uint32), ("h_kv", c_uint32), ("head_dim", c_uint32), ("max_seq", c_uint32)]
+
+
 class WaveInfo(ctypes.Structure):
     """k44b_wave_info_t (include/k44b.h)."""
     _fields_ = [
@@ -100,6 +105,17 @@ PROTOTYPES = {
     "k44b_plan_add_argmax": (c_int, [c_void_p, c_char_p, c_uint64, c_uint32, c_int, c_uint32]),
     "k44b_plan_set_tokens": (c_int, [c_void_p, POINTER(ctypes.c_int32), c_uint32, c_void_p]),
     "k44b_plan_get_next_tokens": (c_int, [c_void_p, POINTER(ctypes.c_int32), c_uint32, c_void_p]),
+    "k44b_plan_add_window_attn": (c_int, [c_void_p, c_char_p, c_uint64, c_uint64, c_uint64, c_uint64, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32,
+                                           c_uint32, c_float, c_int]),
+    "k44b_kv8_bytes": (c_uint64, [c_uint32, c_uint32, c_uint32, c_uint32]),
+    "k44b_kv8_clear": (c_int, [POINTER(KV8CacheDesc), c_void_p]),
+    "k44b_plan_add_kv8_fill": (c_int, [c_void_p, c_char_p, POINTER(KV8CacheDesc), c_uint64, c_uint64, c_uint32, c_float, c_int]),
+    "k44b_plan_set_sequences": (c_int, [c_void_p, POINTER(c_int32), POINTER(c_int32), c_uint32, c_void_p]),
+    "k44b_plan_add_kv8_attn": (c_int, [c_void_p, c_char_p, POINTER(KV8CacheDesc), c_uint64, c_uint64, c_uint64, c_uint64, c_uint32, c_uint32, c_uint32,
+                                        c_float, c_int]),
+    "k44b_plan_set_positions": (c_int, [c_void_p, POINTER(c_int32), c_uint32, c_void_p]),
+    "k44b_plan_add_logprobs": (c_int, [c_void_p, c_char_p, c_uint64, c_uint32, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p]),
+    "k44b_plan_columns": (c_uint32, [c_void_p]),
     "k44b_plan_ipc_handles": (c_int, [c_void_p, c_void_p, c_void_p]),
     "k44b_plan_set_peers_ipc": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "k44b_plan_set_peers_raw": (c_int, [c_void_p, c_int, c_int, POINTER(c_void_p), POINTER(c_void_p)]),

@@ -396,6 +396,87 @@ int k44b_plan_get_next_tokens(void *plan, int32_t *h_tokens, uint32_t n, void *s
     return r == cudaSuccess ? 0 : set_error(std::string("plan_get_next_tokens: ") + cudaGetErrorString(r));
 }
 
+int k44b_plan_add_window_attn(void *plan, const char *name, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off, uint32_t h_q,
+                              uint32_t h_kv, uint32_t head_dim, uint32_t seq_len, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling) {
+    if (!plan) return set_error("plan_add_window_attn: bad arguments");
+    HostWave w;
+    w.kind = AUX_WINDOW_ATTN; w.name = name ? name : "window_attn"; w.cout = h_q * head_dim;
+    w.src_off = q_off; w.src2_off = k_off; w.src3_off = v_off; w.y_off = out_off; w.h_q = h_q; w.h_kv = h_kv; w.head_dim = head_dim;
+    w.seq_len = seq_len; w.window = window; w.sinks = sinks; w.rope_theta = rope_theta; w.llama3_scaling = llama3_scaling != 0;
+    return P(plan)->exec.add_wave(w) ? 0 : set_error(P(plan)->exec.err);
+}
+
+static bool kv8_cache_ok(const k44b_kv8_cache *c, std::string &why) {
+    if (!c || !c->data) { why = "no cache"; return false; }
+    if (c->head_dim != 64u && c->head_dim != 128u) { why = "head_dim must be 64 or 128"; return false; }
+    if (!c->columns || !c->h_kv || !c->max_seq || c->max_seq > 0x7fffffffu) { why = "columns, h_kv and max_seq must not be 0"; return false; }
+    const uint64_t need = k44b_kv8_bytes(c->columns, c->h_kv, c->head_dim, c->max_seq);
+    if (!need || c->bytes < need) { why = "the cache needs " + std::to_string(need) + " bytes"; return false; }
+    return true;
+}
+
+uint64_t k44b_kv8_bytes(uint32_t columns, uint32_t h_kv, uint32_t head_dim, uint32_t max_seq) {
+    if (!columns || !h_kv || !max_seq || max_seq > 0x7fffffffu || (head_dim != 64u && head_dim != 128u)) return 0;
+    if ((uint64_t)columns * h_kv > (1ull << 32)) return 0;                 // far beyond any device; keeps the products below in 64 bits
+    Kv8Cache c;
+    return kv8_layout(c, nullptr, columns, h_kv, head_dim, max_seq);
+}
+
+int k44b_kv8_clear(const k44b_kv8_cache *cache, void *stream) {
+    std::string why;
+    if (!kv8_cache_ok(cache, why)) return set_error("kv8_clear: " + why);
+    Kv8Cache c;
+    const uint64_t bytes = kv8_layout(c, (uint8_t *)cache->data, cache->columns, cache->h_kv, cache->head_dim, cache->max_seq);
+    cudaError_t e = cudaMemsetAsync(cache->data, 0, bytes, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c.tail_block, 0xff, (size_t)cache->columns * cache->h_kv * sizeof(int), (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : set_error(std::string("kv8_clear: ") + cudaGetErrorString(e));
+}
+
+int k44b_plan_add_kv8_fill(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t k_off, uint64_t v_off, uint32_t seq_len, float rope_theta,
+                           int llama3_scaling) {
+    std::string why;
+    if (!plan) return set_error("plan_add_kv8_fill: bad arguments");
+    if (!kv8_cache_ok(cache, why)) return set_error("plan_add_kv8_fill: " + why);
+    HostWave w;
+    w.kind = AUX_KV8_FILL; w.name = name ? name : "kv8_fill"; w.src_off = k_off; w.src2_off = v_off; w.h_kv = cache->h_kv; w.head_dim = cache->head_dim;
+    w.cout = cache->h_kv * cache->head_dim; w.max_seq = cache->max_seq; w.cache_columns = cache->columns; w.cache_data = cache->data; w.seq_len = seq_len;
+    w.rope_theta = rope_theta; w.llama3_scaling = llama3_scaling != 0;
+    return P(plan)->exec.add_wave(w) ? 0 : set_error(P(plan)->exec.err);
+}
+
+int k44b_plan_add_kv8_attn(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off,
+                           uint32_t h_q, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling) {
+    std::string why;
+    if (!plan) return set_error("plan_add_kv8_attn: bad arguments");
+    if (!kv8_cache_ok(cache, why)) return set_error("plan_add_kv8_attn: " + why);
+    HostWave w;
+    w.kind = AUX_KV8_ATTN; w.name = name ? name : "kv8_attn"; w.src_off = q_off; w.src2_off = k_off; w.src3_off = v_off; w.y_off = out_off; w.h_q = h_q;
+    w.h_kv = cache->h_kv; w.head_dim = cache->head_dim; w.cout = h_q * cache->head_dim; w.max_seq = cache->max_seq; w.cache_columns = cache->columns;
+    w.cache_data = cache->data; w.window = window; w.sinks = sinks; w.rope_theta = rope_theta; w.llama3_scaling = llama3_scaling != 0;
+    return P(plan)->exec.add_wave(w) ? 0 : set_error(P(plan)->exec.err);
+}
+
+int k44b_plan_set_positions(void *plan, const int32_t *h_positions, uint32_t n, void *stream) {
+    if (!plan || !h_positions) return set_error("plan_set_positions: bad arguments");
+    return P(plan)->exec.set_positions(h_positions, n, (cudaStream_t)stream) ? 0 : set_error(P(plan)->exec.err);
+}
+
+int k44b_plan_set_sequences(void *plan, const int32_t *h_cache_columns, const int32_t *h_lengths, uint32_t n, void *stream) {
+    if (!plan || !h_cache_columns || !h_lengths) return set_error("plan_set_sequences: bad arguments");
+    return P(plan)->exec.set_sequences(h_cache_columns, h_lengths, n, (cudaStream_t)stream) ? 0 : set_error(P(plan)->exec.err);
+}
+
+int k44b_plan_add_logprobs(void *plan, const char *name, uint64_t src_off, uint32_t rows, const int32_t *d_targets, float *d_logprobs, float *d_entropy,
+                           uint32_t top, int32_t *d_top_rows, float *d_top_logprobs) {
+    if (!plan || !rows) return set_error("plan_add_logprobs: bad arguments");
+    HostWave w;
+    w.kind = AUX_LOGPROBS; w.name = name ? name : "logprobs"; w.cout = rows; w.src_off = src_off; w.targets = d_targets; w.logprobs = d_logprobs;
+    w.entropy = d_entropy; w.top = top; w.top_rows = d_top_rows; w.top_logprobs = d_top_logprobs;
+    return P(plan)->exec.add_wave(w) ? 0 : set_error(P(plan)->exec.err);
+}
+
+uint32_t k44b_plan_columns(void *plan) { return plan ? P(plan)->exec.columns() : 0; }
+
 int k44b_plan_add_image_op(void *plan, int op, const char *name, uint64_t src_off, uint64_t dst_off, uint32_t planes,
                            const k44b_plane_geom *in, const k44b_plane_geom *out) {
     if (!plan || !out || op < AUX_MAXPOOL2 || op > AUX_HALO_CLEAR || (op != AUX_HALO_CLEAR && !in)) return set_error("plan_add_image_op: bad arguments");

@@ -7,7 +7,7 @@ namespace k44b {
 
 const char *status_string(uint32_t st) {
     if (st == 0) return "ok";
-    if (st & ST_BAD_INDEX) return "gather offset outside the canvas";
+    if (st & ST_BAD_INDEX) return "gather offset outside the canvas, or a position or sequence outside its cache";
     if (st & ST_TIMEOUT_PEER) return "timed out waiting for a peer GPU's rows";
     if (st & ST_TIMEOUT_DRAIN) return "timed out draining in-flight copies";
     if (st & ST_TIMEOUT_PRODUCER) return "producer timed out waiting for a free stage";
@@ -216,6 +216,15 @@ void Executor::release() {
     cudaFree(d_next_tokens_); d_next_tokens_ = nullptr;
     cudaFree(d_argmax_); d_argmax_ = nullptr; argmax_words_ = 0;
     cudaFree(d_decode_partial_); d_decode_partial_ = nullptr; decode_partial_bytes_ = 0;
+    for (auto &t : rope_tables_) cudaFree(t.d);
+    rope_tables_.clear();
+    cudaFree(d_positions_); d_positions_ = nullptr;
+    cudaFree(d_sequences_); d_sequences_ = nullptr;
+    h_slots_.clear(); h_lengths_.clear();
+    cudaFree(d_window_); d_window_ = nullptr; window_bytes_ = 0;
+    cudaFree(d_kv8_partial_); d_kv8_partial_ = nullptr; kv8_partial_bytes_ = 0;
+    cudaFree(d_kv8_counters_); d_kv8_counters_ = nullptr; kv8_counter_bytes_ = 0;
+    cudaFree(d_logprob_); d_logprob_ = nullptr; logprob_bytes_ = 0;
     cudaFree(d_sync_); d_sync_ = nullptr;
     cudaFree(d_peers_); d_peers_ = nullptr;
     cudaFree(canvas_); canvas_ = nullptr;
@@ -265,6 +274,11 @@ bool Executor::begin(int device, uint64_t canvas_elems, uint32_t pitch, uint32_t
 // Tensor map over `rows` rows of `pitch_` FP16 elements starting at `base` (a device address valid on this GPU: the own
 // canvas or a peer's mapping), boxes of box_cols x box_rows.
 bool Executor::encode_map(CUtensorMap *map, void *base, uint64_t rows, uint32_t box_cols, uint32_t box_rows, bool swizzle128) {
+    return encode_map_2d(map, base, pitch_, rows, box_cols, box_rows, swizzle128);
+}
+
+// The same over rows of any length: `rows` rows of `inner` FP16 elements.
+bool Executor::encode_map_2d(CUtensorMap *map, void *base, uint64_t inner, uint64_t rows, uint32_t box_cols, uint32_t box_rows, bool swizzle128) {
     typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -276,8 +290,8 @@ bool Executor::encode_map(CUtensorMap *map, void *base, uint64_t rows, uint32_t 
             return fail("cuTensorMapEncodeTiled is not available from the driver");
         encode = (EncodeFn)fn;
     }
-    const cuuint64_t dims[2] = {pitch_, rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)pitch_ * 2u};
+    const cuuint64_t dims[2] = {inner, rows};
+    const cuuint64_t strides[1] = {inner * 2u};
     const cuuint32_t box[2] = {box_cols, box_rows};
     const cuuint32_t estr[2] = {1u, 1u};
     const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -409,6 +423,7 @@ bool Executor::add_aux(const HostWave &w) {
         x.advance = w.advance ? 1u : 0u; x.max_seq = w.max_seq;
         if (!(x.next_tokens = next_tokens_ptr()) || !(x.tokens = tokens_ptr())) return false;
         if (w.advance && !(x.pos_rw = decode_pos_ptr())) return false;
+        x.positions = w.advance ? d_positions_ : nullptr;
         const size_t words = (size_t)((w.cout + kArgmaxChunk - 1u) / kArgmaxChunk) * pitch_;
         if (words > argmax_words_) {
             if (!check(cudaDeviceSynchronize(), "synchronise")) return false;
@@ -451,6 +466,10 @@ bool Executor::add_aux(const HostWave &w) {
         dw.write_lo = w.y_off; dw.write_hi = w.y_off + (uint64_t)dst_planes * go.ch_stride;
         break;
     }
+    case AUX_WINDOW_ATTN: case AUX_KV8_FILL: case AUX_KV8_ATTN: case AUX_LOGPROBS:
+        if (!add_decoder(w, dw)) return false;
+        rlo = dw.read_lo; rhi = dw.read_hi;
+        break;
     default: return fail("unknown command kind");
     }
     dw.read_lo = rlo; dw.read_hi = rhi;
@@ -459,6 +478,218 @@ bool Executor::add_aux(const HostWave &w) {
     drop_graph();
     groups_valid_ = false;
     return true;
+}
+
+// ---- decoder operators (k44_decoder.cuh) -------------------------------------------------------------------------------------
+int *Executor::positions_ptr() {
+    if (!ready()) { fail("executor not initialised"); return nullptr; }
+    if (!d_positions_) {
+        if (!(d_positions_ = alloc_words(device_, pitch_, err))) return nullptr;
+        if (!check(cudaMemset(d_positions_, 0xff, (size_t)pitch_ * sizeof(int)), "positions clear")) return nullptr;      // -1: idle
+        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_ARGMAX && o.aux.advance) o.aux.positions = d_positions_;
+        drop_graph();                               // a graph captured before holds the old arguments
+    }
+    return d_positions_;
+}
+
+int2 *Executor::sequences_ptr() {
+    if (!ready()) { fail("executor not initialised"); return nullptr; }
+    if (!d_sequences_) {
+        int *p = alloc_words(device_, 2u * pitch_, err);
+        if (!p) return nullptr;
+        d_sequences_ = (int2 *)p;
+        if (!check(cudaMemset(p, 0xff, (size_t)pitch_ * sizeof(int2)), "sequence table clear")) return nullptr;            // column -1: skip
+    }
+    return d_sequences_;
+}
+
+bool Executor::set_positions(const int32_t *pos, uint32_t n, cudaStream_t stream) {
+    if (!ready()) return fail("executor not initialised");
+    if (n > columns_) return fail("set_positions: more positions than columns");
+    int32_t most = -1;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (pos[i] < -1) return fail("set_positions: a position is below -1");
+        most = std::max(most, pos[i]);
+    }
+    for (const auto &o : waves_)
+        if (o.is_aux && o.aux.kind == AUX_KV8_ATTN && most >= (int64_t)o.kv8.cache.max_seq) return fail("set_positions: position " + std::to_string(most) + " lies outside the cache of '" + o.name + "'");
+    if (!not_capturing(stream, "set_positions") || !positions_ptr()) return false;
+    // a copy from pageable memory is staged by the runtime before the call returns
+    return check(cudaMemcpyAsync(d_positions_, pos, (size_t)n * sizeof(int32_t), cudaMemcpyHostToDevice, stream), "set_positions");
+}
+
+// Whether the table of sequences fits a fill command: cache columns, lengths, and the columns of the plan they occupy.
+static bool sequences_fit(const Kv8FillArgs &f, const std::vector<int32_t> &slots, const std::vector<int32_t> &lengths, std::string &why) {
+    for (size_t i = 0; i < slots.size(); ++i) {
+        if (slots[i] < 0) continue;
+        if ((uint32_t)slots[i] >= f.cache.columns) { why = "cache column " + std::to_string(slots[i]) + " does not exist"; return false; }
+        if ((uint32_t)lengths[i] > f.seq_len || (uint32_t)lengths[i] > f.cache.max_seq) { why = "length " + std::to_string(lengths[i]) + " exceeds the sequence or the cache"; return false; }
+        if ((uint64_t)i * f.seq_len + (uint32_t)lengths[i] > f.columns) { why = "sequence " + std::to_string(i) + " leaves the plan's columns"; return false; }
+    }
+    return true;
+}
+
+bool Executor::set_sequences(const int32_t *slots, const int32_t *lengths, uint32_t n, cudaStream_t stream) {
+    if (!ready()) return fail("executor not initialised");
+    if (n > pitch_) return fail("set_sequences: more sequences than columns");
+    std::vector<int32_t> s(slots, slots + n), l(lengths, lengths + n), used;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (s[i] < -1 || l[i] < 0) return fail("set_sequences: a cache column below -1 or a negative length");
+        if (s[i] >= 0) used.push_back(s[i]);
+    }
+    std::sort(used.begin(), used.end());
+    if (std::adjacent_find(used.begin(), used.end()) != used.end()) return fail("set_sequences: two sequences name the same cache column");
+    std::string why;
+    for (const auto &o : waves_)
+        if (o.is_aux && o.aux.kind == AUX_KV8_FILL && !sequences_fit(o.fill, s, l, why)) return fail("set_sequences: '" + o.name + "': " + why);
+    if (!not_capturing(stream, "set_sequences") || !sequences_ptr()) return false;
+    std::vector<int2> table(pitch_, make_int2(-1, 0));
+    for (uint32_t i = 0; i < n; ++i) table[i] = make_int2(s[i], l[i]);
+    if (!check(cudaMemcpyAsync(d_sequences_, table.data(), table.size() * sizeof(int2), cudaMemcpyHostToDevice, stream), "set_sequences")) return false;
+    h_slots_ = s; h_lengths_ = l;
+    return true;
+}
+
+// A table of at least `positions` positions; tables live as long as the plan, so that earlier commands keep theirs.
+const float2 *Executor::rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions) {
+    for (const auto &t : rope_tables_)
+        if (t.theta == theta && t.llama3 == llama3 && t.head_dim == head_dim && t.positions >= positions) return t.d;
+    RopeTable t{theta, llama3, head_dim, positions, nullptr};
+    if (!check(cudaMalloc(&t.d, (size_t)positions * (head_dim / 2u) * sizeof(float2)), "rotary table allocation")) return nullptr;
+    if (!check(launch_rope_table(t.d, positions, head_dim, (double)theta, llama3, nullptr), "rotary table") || !check(cudaDeviceSynchronize(), "rotary table")) { cudaFree(t.d); return nullptr; }
+    rope_tables_.push_back(t);
+    return t.d;
+}
+
+// Grows a scratch buffer (cleared); the caller points the commands that use it at the new one. A failure leaves the old one.
+bool Executor::reserve(void *&p, uint64_t &have, uint64_t need, const char *what) {
+    if (need <= have) return true;
+    void *grown = nullptr;
+    if (!check(cudaDeviceSynchronize(), "synchronise") || !check(cudaMalloc(&grown, need), what)) return false;
+    if (!check(cudaMemset(grown, 0, need), what) || !check(cudaDeviceSynchronize(), what)) { cudaFree(grown); return false; }
+    cudaFree(p);
+    p = grown; have = need;
+    return true;
+}
+
+// The small tables that the host sets are copied from pageable memory, which a captured graph would read again later.
+bool Executor::not_capturing(cudaStream_t stream, const char *what) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (!check(cudaStreamIsCapturing(stream, &st), what)) return false;
+    return st == cudaStreamCaptureStatusNone || fail(std::string(what) + " cannot be captured into a graph");
+}
+
+bool Executor::device_memory(const void *p, const char *what) {
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); return fail(std::string(what) + " is not device memory"); }
+    if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == device_)) return true;
+    return fail(std::string(what) + " is not memory of the plan's device");
+}
+
+bool Executor::place_window(DeviceWave &dw) {
+    WindowAttnArgs &a = dw.window;
+    window_attn_place(a, d_window_);
+    auto rows = [&](CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint32_t box_rows) {
+        return encode_map_2d(map, base, inner, outer, 64u, box_rows);
+    };
+    return rows(&dw.window_maps.q, a.q_rows, a.head_dim, (uint64_t)a.h_q * a.pitch, 128u) && rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 128u) &&
+           rows(&dw.window_maps.v, a.v_rows, a.pitch, (uint64_t)a.h_kv * a.head_dim, a.head_dim);
+}
+
+bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
+    auto bad = [&](const std::string &m) { return fail("'" + w.name + "': " + m); };
+    auto inside = [&](uint64_t off, uint64_t rows) { return off % 8u == 0u && off <= canvas_elems_ && rows <= (canvas_elems_ - off) / pitch_; };
+    auto apart = [&](uint64_t x, uint64_t rx, uint64_t y, uint64_t ry) { return x + rx * pitch_ <= y || y + ry * pitch_ <= x; };
+    const unsigned long long wait_cycles = make_umma_desc(64).wait_cycles;
+    dw.read_lo = ~0ull; dw.read_hi = 0; dw.write_lo = 0; dw.write_hi = 0;
+    auto reads = [&](uint64_t off, uint64_t rows) { dw.read_lo = std::min(dw.read_lo, off); dw.read_hi = std::max(dw.read_hi, off + rows * pitch_); };
+    if (w.kind != AUX_LOGPROBS) {
+        if (w.head_dim != 64u && w.head_dim != 128u) return bad("head_dim must be 64 or 128");
+        if (!w.h_kv || w.h_kv > 1024u) return bad("between 1 and 1024 key / value heads are needed");
+        if (!(w.rope_theta > 1.0f) || !std::isfinite(w.rope_theta)) return bad("the rotary base must be a number above 1");
+        if (w.window > 0x7fffffffu || w.sinks > 0x7fffffffu) return bad("window and sinks must be below 2^31");
+    }
+    const uint64_t rk = (uint64_t)w.h_kv * w.head_dim, rq = (uint64_t)w.h_q * w.head_dim;
+    if (w.kind == AUX_WINDOW_ATTN || w.kind == AUX_KV8_ATTN) {
+        if (!w.h_q || w.h_q % w.h_kv || w.h_q > 16384u) return bad("h_q must be a multiple of h_kv");
+        if (!inside(w.src_off, rq) || !inside(w.src2_off, rk) || !inside(w.src3_off, rk) || !inside(w.y_off, rq)) return bad("a tensor leaves the canvas");
+        if (!apart(w.y_off, rq, w.src_off, rq) || !apart(w.y_off, rq, w.src2_off, rk) || !apart(w.y_off, rq, w.src3_off, rk)) return bad("the output overlaps q, k or v");
+        reads(w.src_off, rq); reads(w.src2_off, rk); reads(w.src3_off, rk);
+        dw.write_lo = w.y_off; dw.write_hi = w.y_off + rq * pitch_;
+    }
+    Kv8Cache cache;
+    if (w.kind == AUX_KV8_FILL || w.kind == AUX_KV8_ATTN) {
+        if (!w.cache_data || (uintptr_t)w.cache_data % 256u) return bad("the cache must start on a 256-byte boundary");
+        if (!device_memory(w.cache_data, "the cache")) return bad(err);
+        kv8_layout(cache, (uint8_t *)w.cache_data, w.cache_columns, w.h_kv, w.head_dim, w.max_seq);
+    }
+    switch (w.kind) {
+    case AUX_WINDOW_ATTN: {
+        if (!w.seq_len) return bad("seq_len must not be 0");
+        if ((uint64_t)w.h_q * pitch_ >= 0x7fffffffull || rk * pitch_ >= 0x7fffffffull * 64ull) return bad("too many columns");
+        WindowAttnArgs &a = dw.window;
+        a.q = canvas_ + w.src_off; a.k = canvas_ + w.src2_off; a.v = canvas_ + w.src3_off; a.out = canvas_ + w.y_off;
+        a.pitch = pitch_; a.columns = columns_; a.h_q = w.h_q; a.h_kv = w.h_kv; a.head_dim = w.head_dim; a.seq_len = w.seq_len;
+        a.window = w.window; a.sinks = w.sinks; a.status = d_status_; a.wait_cycles = wait_cycles;
+        if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, std::min(w.seq_len, columns_)))) return false;
+        if (!check(window_attn_setup(), "kernel attribute setup")) return false;
+        const uint64_t need = window_attn_scratch_bytes(pitch_, w.h_q, w.h_kv, w.head_dim);
+        const bool grown = need > window_bytes_;
+        if (!reserve(d_window_, window_bytes_, need, "attention scratch allocation")) return false;
+        if (grown)
+            for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_WINDOW_ATTN && !place_window(o)) return false;
+        return place_window(dw);
+    }
+    case AUX_KV8_FILL: {
+        if (!inside(w.src_off, rk) || !inside(w.src2_off, rk)) return bad("a tensor leaves the canvas");
+        if (!w.seq_len) return bad("seq_len must not be 0");
+        reads(w.src_off, rk); reads(w.src2_off, rk);
+        Kv8FillArgs &a = dw.fill;
+        a.cache = cache; a.k = canvas_ + w.src_off; a.v = canvas_ + w.src2_off;
+        a.pitch = pitch_; a.columns = columns_; a.seq_len = w.seq_len; a.status = d_status_;
+        if ((columns_ + w.seq_len - 1u) / w.seq_len > 65535u) return bad("too many sequences");
+        if (!(a.sequences = sequences_ptr())) return false;
+        std::string why;
+        if (!sequences_fit(a, h_slots_, h_lengths_, why)) return bad("the sequences set before do not fit: " + why);
+        if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, std::min(w.seq_len, w.max_seq)))) return false;
+        return true;
+    }
+    case AUX_KV8_ATTN: {
+        if (w.h_q / w.h_kv > 16u) return bad("at most 16 query heads per key / value head");
+        if (w.cache_columns < columns_) return bad("the cache has fewer columns than the plan");
+        if (columns_ > kKv8MaxColumns) return bad("at most " + std::to_string(kKv8MaxColumns) + " columns");
+        if ((uint64_t)columns_ * w.h_kv * (cache.blocks + 1ull) >= 0xffffffffull) return bad("the cache is too large");
+        Kv8AttnArgs &a = dw.kv8;
+        a.cache = cache; a.q = canvas_ + w.src_off; a.k = canvas_ + w.src2_off; a.v = canvas_ + w.src3_off; a.out = canvas_ + w.y_off;
+        a.pitch = pitch_; a.columns = columns_; a.h_q = w.h_q; a.window = w.window; a.sinks = w.sinks; a.status = d_status_; a.wait_cycles = wait_cycles;
+        if (!(a.positions = positions_ptr())) return false;
+        if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, w.max_seq))) return false;
+        if (!check(kv8_attn_setup(), "kernel attribute setup")) return false;
+        if (!reserve(d_kv8_partial_, kv8_partial_bytes_, kv8_attn_partial_bytes((uint32_t)num_sms_, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") ||
+            !reserve(d_kv8_counters_, kv8_counter_bytes_, (uint64_t)columns_ * w.h_kv * sizeof(uint32_t), "attention scratch allocation")) return false;
+        a.partial = (float *)d_kv8_partial_; a.counters = (uint32_t *)d_kv8_counters_;
+        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_KV8_ATTN) { o.kv8.partial = a.partial; o.kv8.counters = a.counters; }
+        return true;
+    }
+    case AUX_LOGPROBS: {
+        if (!w.cout || w.cout > kLogprobMaxRows || !inside(w.src_off, w.cout)) return bad("the logits leave the canvas, or have too many rows");
+        if (w.top > kLogprobTop || w.top > w.cout) return bad("at most " + std::to_string(kLogprobTop) + " alternatives, and no more than rows");
+        if ((w.logprobs != nullptr) != (w.targets != nullptr)) return bad("targets and logprobs go together");
+        if (w.top && (!w.top_rows || !w.top_logprobs)) return bad("alternatives need both of their arrays");
+        if (!w.logprobs && !w.entropy && !w.top) return bad("nothing is asked for");
+        const std::pair<const void *, const char *> arrays[] = {{w.targets, "targets"}, {w.logprobs, "logprobs"}, {w.entropy, "entropy"}, {w.top ? (const void *)w.top_rows : nullptr, "top_rows"}, {w.top ? (const void *)w.top_logprobs : nullptr, "top_logprobs"}};
+        for (const auto &p : arrays) if (p.first && !device_memory(p.first, p.second)) return bad(err);
+        reads(w.src_off, w.cout);
+        LogprobArgs &a = dw.logprob;
+        a.x = canvas_ + w.src_off; a.rows = w.cout; a.pitch = pitch_; a.columns = columns_; a.top = w.top;
+        a.targets = w.targets; a.logprobs = w.logprobs; a.entropy = w.entropy; a.top_rows = w.top_rows; a.top_logprobs = w.top_logprobs;
+        if (!reserve(d_logprob_, logprob_bytes_, logprob_scratch_bytes(w.cout, columns_), "probability scratch allocation")) return false;
+        logprob_place(a, d_logprob_);
+        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_LOGPROBS) logprob_place(o.logprob, d_logprob_);
+        return true;
+    }
+    default: return fail("unknown command kind");
+    }
 }
 
 // A wave over 2-D image planes (convolution taps as element offsets relative to per-tile anchors, outputs at per-tile plane
@@ -970,8 +1201,16 @@ bool Executor::launch_one(DeviceWave &w, cudaStream_t stream, uint32_t peer_slac
     cudaError_t e;
     w.args.peer_slack = peer_slack;
     if (w.is_aux) {
+        const std::string what = "launch of '" + w.name + "'";
+        switch (w.aux.kind) {
+        case AUX_WINDOW_ATTN: launches_ += 2u; return check(launch_window_attn(w.window, w.window_maps, pdl_, stream), what.c_str());
+        case AUX_KV8_FILL: ++launches_; return check(launch_kv8_fill(w.fill, pdl_, stream), what.c_str());
+        case AUX_KV8_ATTN: ++launches_; return check(launch_kv8_attn(w.kv8, (uint32_t)num_sms_, pdl_, stream), what.c_str());
+        case AUX_LOGPROBS: launches_ += 2u; return check(launch_logprobs(w.logprob, pdl_, stream), what.c_str());
+        default: break;
+        }
         launches_ += (w.aux.kind == AUX_ROPE_ATTN || w.aux.kind == AUX_DECODE_ATTN) ? 3u : (w.aux.kind == AUX_ARGMAX ? 2u : 1u);
-        return check(launch_aux(w.aux, pdl_, stream), ("launch of '" + w.name + "'").c_str());
+        return check(launch_aux(w.aux, pdl_, stream), what.c_str());
     }
     if (w.path == PATH_UMMA && w.use_cluster) {
         WaveGroupArgs g;
@@ -1119,6 +1358,7 @@ void Executor::recover_after_abort() {
     if (d_scratch_) cudaMemset(d_scratch_, 0, scratch_tiles_ * 64u * kTileM * sizeof(float));
     if (d_counters_) cudaMemset(d_counters_, 0, scratch_tiles_ * sizeof(uint32_t));
     if (d_sync_) cudaMemset(d_sync_ + kSyncDone, 0, sizeof(uint32_t));
+    if (d_kv8_counters_) cudaMemset(d_kv8_counters_, 0, kv8_counter_bytes_);
     cudaDeviceSynchronize();
 }
 

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "k44_host.hpp"
+#include "k44_decoder.cuh"
 #include "k44_kernels.cuh"
 
 namespace k44b {
@@ -41,6 +42,11 @@ struct DeviceWave {
     std::string name;
     bool is_aux = false;                 // element-wise / attention step (k44_valu.cu) instead of a wave
     AuxArgs aux;
+    WindowAttnArgs window;               // aux.kind 13: prompt attention with a window and sinks
+    WindowAttnMaps window_maps;
+    Kv8FillArgs fill;                    // 14: prompt keys / values into an 8-bit cache
+    Kv8AttnArgs kv8;                     // 15: single tokens against it
+    LogprobArgs logprob;                 // 16: answer probabilities
     WaveArgs args;
     UmmaDesc desc;
     CUtensorMap tmap;
@@ -71,6 +77,11 @@ class Executor {
     bool add_wave(const HostWave &w);
     bool add_aux(const HostWave &w);                               // HostWave::kind != 0
     bool add_wave_2d(const HostWave &w);                           // HostWave::pitch2d != 0: a wave over image planes
+    bool add_decoder(const HostWave &w, DeviceWave &dw);           // kinds 13 .. 16
+    int *positions_ptr();                                          // device int32 [pitch]: position of each column's new token, -1 idle
+    int2 *sequences_ptr();                                         // device int2 [pitch]: per sequence of a prompt plan (cache column or -1, length)
+    bool set_positions(const int32_t *pos, uint32_t n, cudaStream_t stream);
+    bool set_sequences(const int32_t *slots, const int32_t *lengths, uint32_t n, cudaStream_t stream);
     int *tokens_ptr();                                             // device int32 [pitch]: token id per column (embedding gather input)
     int *next_tokens_ptr();                                        // device int32 [pitch]: result of the last arg-max command
     int *decode_pos_ptr();                                         // device word holding the position decode attention works at
@@ -112,6 +123,7 @@ class Executor {
     const DeviceWave &wave(size_t i) const { return waves_[i]; }
     int device() const { return device_; }
     uint32_t pitch() const { return pitch_; }
+    uint32_t columns() const { return columns_; }
     uint64_t launches() const { return launches_; }
 
   private:
@@ -119,8 +131,14 @@ class Executor {
     bool check(cudaError_t e, const char *what);
     bool make_tensor_map(DeviceWave &dw, uint32_t box_cols, bool swizzle128);
     bool encode_map(CUtensorMap *map, void *base, uint64_t rows, uint32_t box_cols, uint32_t box_rows, bool swizzle128);
+    bool encode_map_2d(CUtensorMap *map, void *base, uint64_t inner, uint64_t rows, uint32_t box_cols, uint32_t box_rows, bool swizzle128 = true);
     bool upload_out_maps(DeviceWave &dw, void *const *peer_canvases, uint32_t n);
     bool reserve_scratch(size_t tiles);
+    const float2 *rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions);
+    bool place_window(DeviceWave &dw);
+    bool reserve(void *&p, uint64_t &have, uint64_t need, const char *what);
+    bool device_memory(const void *p, const char *what);
+    bool not_capturing(cudaStream_t stream, const char *what);
     void recover_after_abort();
     bool launch_one(DeviceWave &w, cudaStream_t stream, uint32_t peer_slack = 0);
     void drop_graph();
@@ -154,6 +172,14 @@ class Executor {
     size_t argmax_words_ = 0;
     float *d_decode_partial_ = nullptr;   // per-chunk partial attention results, shared by all decode-attention commands
     size_t decode_partial_bytes_ = 0;
+    // decoder operators: tables and scratch shared by all commands of the plan (they run one after the other)
+    struct RopeTable { float theta; bool llama3; uint32_t head_dim, positions; float2 *d; };
+    std::vector<RopeTable> rope_tables_;
+    int *d_positions_ = nullptr;
+    int2 *d_sequences_ = nullptr;
+    std::vector<int32_t> h_slots_, h_lengths_;      // what set_sequences was given last
+    void *d_window_ = nullptr, *d_kv8_partial_ = nullptr, *d_kv8_counters_ = nullptr, *d_logprob_ = nullptr;
+    uint64_t window_bytes_ = 0, kv8_partial_bytes_ = 0, kv8_counter_bytes_ = 0, logprob_bytes_ = 0;
     // neuron sharding over several GPUs (see PeerArgs)
     uint32_t *d_sync_ = nullptr;          // kSyncWords words, allocated on first use
     PeerArgs *d_peers_ = nullptr;

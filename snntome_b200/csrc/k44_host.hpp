@@ -273,6 +273,13 @@ struct HostWave {
     float eps = 1e-5f, rope_theta = 10000.0f;
     uint32_t h_q = 0, h_kv = 0, head_dim = 0, seq_len = 0, max_seq = 0;
     bool llama3_scaling = false;
+    // Decoder operators (kinds 13..16, k44_decoder.cuh): 13 prompt attention with a window and sinks, 14 filling an 8-bit cache,
+    // 15 single tokens against it, 16 answer probabilities. The cache and the arrays of kind 16 belong to the caller.
+    uint32_t window = 0, sinks = 0, cache_columns = 0, top = 0;
+    void *cache_data = nullptr;
+    const int32_t *targets = nullptr;
+    float *logprobs = nullptr, *entropy = nullptr, *top_logprobs = nullptr;
+    int32_t *top_rows = nullptr;
     // 2-D image waves and commands (kinds 7..12): the layout of the tensor the tiles walk over. pitch2d != 0 marks them:
     // rows are `pitch2d` (a plane's channel stride) apart instead of the plan's row pitch, and tile t reads from
     // tile_off_x[t] and writes to tile_off_y[t] (packed with a quad mask when `tile_mask`), see Layout2D.

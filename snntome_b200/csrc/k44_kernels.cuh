@@ -122,6 +122,7 @@ struct AuxArgs {
     const __half *table = nullptr;
     uint32_t vocab = 0, advance = 0;
     int *tokens = nullptr, *next_tokens = nullptr, *pos_rw = nullptr;
+    int *positions = nullptr;                                        // per-column positions of the 8-bit cache's columns, moved on with pos_rw
     unsigned long long *argmax_scratch = nullptr;                    // [row chunks][pitch] packed (value key, row)
     // 2-D image commands: `rows` planes; source / destination geometry (pixels, padded row length, plane stride)
     uint32_t h_in = 0, w_in = 0, wpad_in = 0, cs_in = 0, h_out = 0, w_out = 0, wpad_out = 0, cs_out = 0;

@@ -472,6 +472,10 @@ __global__ void __launch_bounds__(256) k44_valu_argmax_final_kernel(const AuxArg
         const int row = (int)(0xffffffffu - (uint32_t)(best & 0xffffffffull));
         a.next_tokens[col] = row;
         if (a.advance && col < a.columns) a.tokens[col] = row;
+        if (a.advance && a.positions && col < a.columns) {             // a column at a position of its own; idle columns stay idle
+            const int p = a.positions[col];
+            if (p >= 0) a.positions[col] = (a.max_seq && p + 1 >= (int)a.max_seq) ? (int)a.max_seq - 1 : p + 1;
+        }
     }
     if (a.advance && col == 0u && a.pos_rw) {
         const int p = *a.pos_rw;

@@ -1,0 +1,383 @@
+// Prompt attention with a sliding window and sinks: rotary embedding and causal grouped-query attention of every sequence of a
+// prompt plan (blocks of seq_len columns, any length), on the fifth-generation tensor cores.
+//
+//   visible(t, c):  s0 <= c <= t  and  (window == 0  or  c > t - window  or  c < s0 + sinks),   s0 = first column of t's sequence
+//   o_t = sum_c softmax_c(q_t . k_c / sqrt(D)) v_c
+//
+// Two launches. The first rotates q and k and lays them out token by token (the rows a tensor-core operand wants), and copies v;
+// q, k and v on the canvas stay as they are. The second is the attention: a CTA owns 128 columns of one query head and walks
+// the tiles of 128 keys that any of its columns sees — hidden tiles are never read. Tiles are cut at multiples of 128 canvas
+// columns whatever the sequences' lengths, so that every copy is aligned; sequences that end inside a tile cost a mask.
+#include "k44_decoder.cuh"
+#include "k44_ptx.cuh"
+
+namespace k44b {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) != 0x7c00u; }
+
+// ---- operands ---------------------------------------------------------------------------------------------------------------
+// CTA = 64 columns of one head of q, k or v. Columns behind the plan's last one become zero. Values that are not finite become
+// zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the tensor cores;
+// the attention adds them to the columns that do see them.
+template <int D>
+__global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a) {
+    dep_enter();
+    constexpr int ROW = 64 + 8;
+    __shared__ __align__(16) __half xs[D * ROW];
+    const uint32_t tile = blockIdx.x, tid = threadIdx.x, col0 = tile * 64u;
+    uint32_t h = blockIdx.y;
+    if (h >= a.h_q + a.h_kv) {
+        h -= a.h_q + a.h_kv;
+        const __half *src = a.v + (uint64_t)h * D * a.pitch + col0;
+        __half *dst = a.v_rows + (uint64_t)h * D * a.pitch + col0;
+        uint32_t bad = 0;
+        for (uint32_t e = tid; e < D * 8u; e += 256u) {
+            const uint32_t d = e >> 3, c = (e & 7u) * 8u;
+            uint4 x = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
+            uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t c0 = col0 + c + 2u * i;
+                uint32_t keep = (c0 < a.columns ? 0xffffu : 0u) | (c0 + 1u < a.columns ? 0xffff0000u : 0u);
+                w[i] &= keep;
+                if (!finite_bits(w[i])) { bad = 1u; w[i] &= 0xffff0000u; }
+                if (!finite_bits(w[i] >> 16)) { bad = 1u; w[i] &= 0xffffu; }
+            }
+            *reinterpret_cast<uint4 *>(dst + (uint64_t)d * a.pitch + c) = x;
+        }
+        const int any = __syncthreads_or((int)bad);
+        if (tid == 0u) a.v_flags[h * (a.pitch / 64u) + tile] = any ? 1u : 0u;
+        return;
+    }
+    const bool is_q = h < a.h_q;
+    if (!is_q) h -= a.h_q;
+    const __half *src = (is_q ? a.q : a.k) + (uint64_t)h * D * a.pitch + col0;
+    __half *dst = (is_q ? a.q_rows : a.k_rows) + ((uint64_t)h * a.pitch + col0) * D;
+    for (uint32_t e = tid; e < D * 8u; e += 256u) {
+        const uint32_t d = e >> 3, c = (e & 7u) * 8u;
+        *reinterpret_cast<uint4 *>(xs + d * ROW + c) = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
+    }
+    __syncthreads();
+    // a thread owns one token and runs of 8 pairs: 16 bytes of either half of the row
+    const uint32_t tok = tid & 63u, col = col0 + tok;
+    const bool live = col < a.columns;
+    const float2 *cs = a.rope + (uint64_t)(col % a.seq_len) * (D / 2);
+    for (uint32_t p0 = (tid >> 6) * 8u; p0 < D / 2; p0 += 32u) {
+        __half lo[8], hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = __half2float(xs[(p0 + i) * ROW + tok]), y = __half2float(xs[(p0 + i + D / 2) * ROW + tok]);
+            const float2 r = live ? __ldg(cs + p0 + i) : make_float2(0.f, 0.f);
+            lo[i] = __float2half_rn(live ? x * r.x - y * r.y : 0.f);
+            hi[i] = __float2half_rn(live ? x * r.y + y * r.x : 0.f);
+        }
+        *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0) = *reinterpret_cast<uint4 *>(lo);
+        *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0 + D / 2) = *reinterpret_cast<uint4 *>(hi);
+    }
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------------------
+// Warp 0 copies (TMA), one thread of warp 1 issues the MMAs, warps 2-5 are the softmax: a thread owns one column (= TMEM lane).
+// Tensor memory: 128 columns of scores, over whose first half the weights are written as FP16 pairs once they are read (the A
+// operand of the second product), and D columns of output. That is half of the SM's, so two CTAs share an SM and one's
+// exponentials run under the other's products: per tile 128 x 128 exponentials take 1024 cycles of the SM's 16 per cycle, the
+// products 256 (D = 64) — the exponentials bound this kernel, not the tensor cores.
+// The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
+// exact in FP16 as weights up to 1, and the sum is kept against the same maximum.
+template <int D> struct Shape {
+    static constexpr uint32_t HF = D / 64;
+    static constexpr uint32_t Q_BYTES = 128u * D * 2u, K_BYTES = Q_BYTES, V_BYTES = Q_BYTES;
+    static constexpr uint32_t STAGES = D == 64 ? 2u : 1u;
+    static constexpr uint32_t SMEM = Q_BYTES + STAGES * (K_BYTES + V_BYTES) + 1024u + 256u;
+};
+constexpr uint32_t kThreads = 192, kTmemCols = 256, kOCol = 128;
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    // K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2)
+k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const WindowAttnArgs a) {
+    using S = Shape<D>;
+    constexpr uint32_t HF = S::HF, ST = S::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q_smem = base, k_smem = q_smem + S::Q_BYTES, v_smem = k_smem + ST * S::K_BYTES, ctl = v_smem + ST * S::V_BYTES;
+    const uint32_t q_full = ctl, k_full = ctl + 8u, k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST;
+    const uint32_t s_full = v_empty + 8u * ST, p_full = s_full + 8u, o_full = p_full + 8u;
+    uint8_t *ctl_ptr = smem_raw + (ctl - ptx::smem_addr(smem_raw));
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(ctl_ptr + 128), *abort_word = tmem_slot + 1;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(q_full, 1);
+        for (uint32_t s = 0; s < ST; ++s) {
+            ptx::mbar_init(k_full + 8u * s, 1); ptx::mbar_init(k_empty + 8u * s, 1);
+            ptx::mbar_init(v_full + 8u * s, 1); ptx::mbar_init(v_empty + 8u * s, 1);
+        }
+        ptx::mbar_init(s_full, 1); ptx::mbar_init(p_full, 128); ptx::mbar_init(o_full, 1);
+        *abort_word = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_addr(const_cast<uint32_t *>(tmem_slot)), kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dep_enter();
+    auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        const long long t0 = clock64();
+        for (uint32_t it = 0;; ++it) {
+            if (ptx::mbar_try_wait(bar, parity)) return true;
+            if ((it & 31u) == 31u) {
+                if (*abort_word != 0u) return false;
+                if ((unsigned long long)(clock64() - t0) > a.wait_cycles) return false;
+            }
+        }
+    };
+    // ---- which tiles of keys ----
+    const uint32_t hq = blockIdx.x, qt = gridDim.y - 1u - blockIdx.y, hk = hq / (a.h_q / a.h_kv);      // the longest rows first
+    const uint32_t t_first = qt * 128u, t_last = min(t_first + 127u, a.columns - 1u);
+    const uint32_t s_first = t_first / a.seq_len * a.seq_len;                       // start of the first column's sequence
+    const bool one_seq = t_last - s_first < a.seq_len;
+    uint32_t lo_first = s_first;
+    if (a.window && t_first - s_first >= a.window) lo_first = t_first - a.window + 1u;
+    const uint32_t w_tile = lo_first / 128u;
+    uint32_t n_sink = 0, sink_tile = s_first / 128u;
+    if (a.window && a.sinks && sink_tile < w_tile) n_sink = min(w_tile, (s_first + min(a.sinks, a.seq_len) - 1u) / 128u + 1u) - sink_tile;
+    const uint32_t n = n_sink + (qt - w_tile + 1u);
+    auto key_tile = [&](uint32_t j) -> uint32_t { return j < n_sink ? sink_tile + j : w_tile + (j - n_sink); };
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t keep = ptx::policy_evict_last();
+            ptx::mbar_arrive_expect_tx(q_full, S::Q_BYTES);
+            for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(q_smem + f * 16384u, &q_map, (int32_t)(64u * f), (int32_t)(hq * a.pitch + t_first), q_full, keep);
+            uint32_t k_issued = 0, v_issued = 0;
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t s = j % ST, ph = (j / ST) & 1u, c0 = key_tile(j) * 128u;
+                if (!(ok = wait(k_empty + 8u * s, ph ^ 1u))) break;
+                ptx::mbar_arrive_expect_tx(k_full + 8u * s, S::K_BYTES);
+                for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(k_smem + s * S::K_BYTES + f * 16384u, &k_map, (int32_t)(64u * f), (int32_t)(hk * a.pitch + c0), k_full + 8u * s, keep);
+                ++k_issued;
+                if (!(ok = wait(v_empty + 8u * s, ph ^ 1u))) break;
+                ptx::mbar_arrive_expect_tx(v_full + 8u * s, S::V_BYTES);
+                for (uint32_t f = 0; f < 2u; ++f) ptx::tma_load_2d(v_smem + s * S::V_BYTES + f * (D * 128u), &v_map, (int32_t)(c0 + 64u * f), (int32_t)(hk * D), v_full + 8u * s, keep);
+                ++v_issued;
+            }
+            if (!ok) {
+                if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_PRODUCER);
+                *abort_word = 1u;
+                // wait (bounded) for this CTA's copies in flight before its shared memory goes away
+                auto drain = [&](uint32_t bar, uint32_t parity) {
+                    const long long t0 = clock64();
+                    bool done = false;
+                    while (!done && (unsigned long long)(clock64() - t0) < a.wait_cycles) done = ptx::mbar_try_wait(bar, parity);
+                    if (!done) atomicOr(a.status, (uint32_t)ST_TIMEOUT_DRAIN);
+                };
+                drain(q_full, 0u);
+                for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) drain(k_full + 8u * (i % ST), (i / ST) & 1u);
+                for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) drain(v_full + 8u * (i % ST), (i / ST) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+            ok = wait(q_full, 0u);
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                const uint32_t s = j % ST, ph = (j / ST) & 1u;
+                if (!(ok = wait(k_full + 8u * s, ph))) break;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < D / 16u; ++k)
+                    ptx::umma_f16(tmem, desc_sw128(q_smem + (k >> 2) * 16384u) + (k & 3u) * 2u, desc_sw128(k_smem + s * S::K_BYTES + (k >> 2) * 16384u) + (k & 3u) * 2u, idesc_s, k != 0u ? 1u : 0u);
+                ptx::umma_commit(k_empty + 8u * s);
+                ptx::umma_commit(s_full);
+                if (!(ok = wait(v_full + 8u * s, ph) && wait(p_full, j & 1u))) break;
+                ptx::tc_fence_after();
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k)
+                    ptx::umma_f16_a_tmem(tmem + kOCol, tmem + 8u * k, desc_sw128(v_smem + s * S::V_BYTES + (k >> 2) * (D * 128u)) + (k & 3u) * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
+                ptx::umma_commit(v_empty + 8u * s);
+                if (j + 1u == n) ptx::umma_commit(o_full);
+            }
+            if (!ok) {
+                if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_MMA);
+                *abort_word = 1u;
+            }
+        }
+        __syncwarp();
+    } else {
+        const uint32_t quarter = warp & 3u, row = quarter * 32u + lane, t = t_first + row;
+        const uint32_t lane_base = tmem + ((quarter * 32u) << 16);
+        const float mul = rsqrtf((float)D) * kLog2e;
+        // what column t sees: [lo, t] and [s0, s0 + sk)
+        const uint32_t s0 = t / a.seq_len * a.seq_len;
+        const uint32_t lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0, span = t - lo + 1u;
+        const uint32_t sk = lo > s0 ? min(a.sinks, lo - s0) : 0u;
+        float m = -INFINITY, l = 0.f;                                     // maximum that the weights are kept against (scaled), their sum
+        for (uint32_t j = 0; j < n && ok; ++j) {
+            const uint32_t c0 = key_tile(j) * 128u;
+            // nothing to hide: all keys before all columns, inside every column's window (or among the sinks), one sequence
+            const bool whole = one_seq && c0 + 127u <= t_first && c0 >= s_first &&
+                               (a.window == 0u || t_first + 127u < c0 + a.window || c0 + 128u <= s_first + a.sinks);
+            ok = __all_sync(0xffffffffu, wait(s_full, j & 1u) ? 1 : 0) != 0;
+            if (!ok) break;
+            ptx::tc_fence_after();
+            float mx = -INFINITY;
+            uint32_t r[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32(lane_base + 32u * q, r[q]);
+            ptx::tmem_ld_wait();
+            if (!whole) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const uint32_t c = c0 + 32u * q + i;
+                        if (!(c - lo < span || c - s0 < sk)) r[q][i] = 0xff800000u;
+                    }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[q][i]));
+            mx *= mul;
+            if (__any_sync(0xffffffffu, mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY))) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+                m = mn;
+                l *= f;
+                if (j != 0u) {
+#pragma unroll 1
+                    for (uint32_t d0 = 0; d0 < D; d0 += 32u) {
+                        uint32_t o[32];
+                        ptx::tmem_ld_32x32(lane_base + kOCol + d0, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        ptx::tmem_st_32x32(lane_base + kOCol + d0, o);
+                    }
+                }
+            }
+            const float shift = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = fast_exp2(fmaf(__uint_as_float(r[2 * q + (i >> 4)][2 * (i & 15)]), mul, -shift));
+                    const float y = fast_exp2(fmaf(__uint_as_float(r[2 * q + (i >> 4)][2 * (i & 15) + 1]), mul, -shift));
+                    sum[(2 * i) & 3] += x;
+                    sum[(2 * i + 1) & 3] += y;
+                    const __half2 h = __floats2half2_rn(x, y);
+                    p[i] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+                ptx::tmem_st_32x32(lane_base + 32u * q, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(p_full);
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait(o_full, 0u) ? 1 : 0) != 0;
+        if (ok) {
+            ptx::tc_fence_after();
+            const float inv = 1.0f / l;
+            // values that were kept from the tensor cores: a column that sees one gets it
+            bool flagged = false;
+            const uint32_t *flags = a.v_flags + hk * (a.pitch / 64u);
+            for (uint32_t j = 0; j < n; ++j) {
+                const uint32_t f = key_tile(j) * 2u;
+                flagged |= flags[f] != 0u || (f + 1u < a.pitch / 64u && flags[f + 1u] != 0u);
+            }
+            __half *dst = a.out + (uint64_t)hq * D * a.pitch + t;
+#pragma unroll 1
+            for (uint32_t d0 = 0; d0 < D; d0 += 32u) {
+                uint32_t o[32];
+                ptx::tmem_ld_32x32(lane_base + kOCol + d0, o);
+                ptx::tmem_ld_wait();
+                if (flagged && t < a.columns) {
+                    for (uint32_t j = 0; j < n; ++j) {
+                        const uint32_t c0 = key_tile(j) * 128u;
+                        for (uint32_t c = c0; c < c0 + 128u && c <= t; ++c) {
+                            if (!(c - lo < span || c - s0 < sk)) continue;
+                            const __half *col = a.v + ((uint64_t)hk * D + d0) * a.pitch + c;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const __half v = col[(uint64_t)i * a.pitch];
+                                if (!finite_bits(__half_as_ushort(v))) o[i] = __float_as_uint(__uint_as_float(o[i]) + __half2float(v));
+                            }
+                        }
+                    }
+                }
+                if (t < a.columns) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) dst[(uint64_t)(d0 + i) * a.pitch] = __float2half_rn(__uint_as_float(o[i]) * inv);
+                }
+            }
+        } else if (lane == 0) {
+            if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_EPILOGUE);
+            *abort_word = 1u;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    if (warp == 1) ptx::tmem_dealloc(tmem, kTmemCols);
+}
+
+}  // namespace
+
+uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_q, uint32_t h_kv, uint32_t head_dim) {
+    const uint64_t row = (uint64_t)pitch * head_dim * 2u;
+    return kv8_align(h_q * row) + 2u * kv8_align(h_kv * row) + kv8_align((uint64_t)h_kv * (pitch / 64u) * 4u);
+}
+
+void window_attn_place(WindowAttnArgs &a, void *scratch) {
+    const uint64_t row = (uint64_t)a.pitch * a.head_dim * 2u;
+    uint8_t *p = (uint8_t *)scratch;
+    a.q_rows = (__half *)p; p += kv8_align(a.h_q * row);
+    a.k_rows = (__half *)p; p += kv8_align(a.h_kv * row);
+    a.v_rows = (__half *)p; p += kv8_align(a.h_kv * row);
+    a.v_flags = (uint32_t *)p;
+}
+
+cudaError_t window_attn_setup() {
+    cudaError_t e = cudaFuncSetAttribute(k44_window_attn_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<64>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k44_window_attn_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<128>::SMEM);
+    return e;
+}
+
+cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m, bool pdl, cudaStream_t s) {
+    // operands for whole tiles of 128 columns (what lies behind the last column is zero, not whatever the scratch held)
+    const uint32_t tiles = (a.columns + 127u) / 128u;
+    const dim3 g1(std::min(2u * tiles, a.pitch / 64u), a.h_q + 2u * a.h_kv), g2(a.h_q, tiles);
+    cudaError_t e;
+    if (a.head_dim == 64u) {
+        e = launch_dep(k44_window_operands_kernel<64>, g1, dim3(256), 0, pdl, s, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.q, m.k, m.v, a);
+    } else {
+        e = launch_dep(k44_window_operands_kernel<128>, g1, dim3(256), 0, pdl, s, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.q, m.k, m.v, a);
+    }
+    return e;
+}
+
+}  // namespace k44b

@@ -7,7 +7,7 @@ from typing import Optional
 
 import numpy as np
 
-from ._lib import PlaneGeom, WaveDesc, WaveInfo, get_lib, last_error
+from ._lib import KV8CacheDesc, PlaneGeom, WaveDesc, WaveInfo, get_lib, last_error
 from .plan import Plan, Wave
 
 PATH_AUTO, PATH_FMA, PATH_UMMA = -1, 0, 1
@@ -63,12 +63,100 @@ def wave_desc(w: Wave, *, device_weights_ptr: int = 0, run_rows: Optional[np.nda
     return d, keep
 
 
+class KV8Cache:
+    """Key / value cache of 8 bits for `columns` sequences of up to `max_seq` positions (include/k44b.h): e4m3 codes in blocks of 64
+    positions with one FP32 scale per block, head and column for keys and for values, and the open block as FP16 rows. The storage is
+    a uint8 CUDA tensor, allocated and cleared here unless given; a prompt plan fills it (`add_kv8_fill`), a decode plan reads it
+    (`add_kv8_attn`)."""
+
+    BLOCK = 64
+
+    def __init__(self, columns: int, h_kv: int, head_dim: int, max_seq: int, device: int = 0, storage=None):
+        import torch
+        for what, v in (("columns", columns), ("h_kv", h_kv), ("max_seq", max_seq)):
+            if not 0 < int(v) < 1 << 31:
+                raise NativeError(f"KV8Cache: {what} must be between 1 and 2^31 - 1")
+        self.columns, self.h_kv, self.head_dim, self.max_seq = int(columns), int(h_kv), int(head_dim), int(max_seq)
+        need = self.bytes_needed(columns, h_kv, head_dim, max_seq)
+        if need == 0:
+            raise NativeError("KV8Cache: head_dim must be 64 or 128, and the sizes must fit a device")
+        fresh = storage is None
+        if fresh:
+            storage = torch.empty(need, dtype=torch.uint8, device=f"cuda:{int(device)}")
+        if storage.dtype != torch.uint8 or not storage.is_cuda or not storage.is_contiguous() or storage.numel() < need or storage.data_ptr() % 256:
+            raise NativeError(f"KV8Cache: the storage must be {need} contiguous bytes (uint8) of device memory on a 256-byte boundary")
+        self.storage = storage
+        self._desc = KV8CacheDesc(storage.data_ptr(), storage.numel(), self.columns, self.h_kv, self.head_dim, self.max_seq)
+        if fresh:
+            self.clear()
+
+    @staticmethod
+    def bytes_needed(columns: int, h_kv: int, head_dim: int, max_seq: int) -> int:
+        return int(get_lib().k44b_kv8_bytes(int(columns), int(h_kv), int(head_dim), int(max_seq)))
+
+    @property
+    def blocks(self) -> int:
+        return (self.max_seq + self.BLOCK - 1) // self.BLOCK
+
+    def clear(self, stream=None) -> None:
+        """Empty every column (on `stream`, default torch's current stream of the storage's device)."""
+        import torch
+        if stream is None:
+            stream = torch.cuda.current_stream(self.storage.device)
+        sp = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+        with torch.cuda.device(self.storage.device):
+            if get_lib().k44b_kv8_clear(ctypes.byref(self._desc), ctypes.c_void_p(sp)) != 0:
+                raise NativeError(f"kv8_clear: {last_error()}")
+
+    def views(self) -> dict:
+        """The parts of the storage as tensors: codes [column, head, block, 2, 64 * head_dim] (e4m3), scales [column, head, block, 2],
+        k_tail [column, head, 64, head_dim], v_tail [column, head, head_dim, 64], tail_block [column, head]."""
+        import torch
+        c, h, d, nb = self.columns, self.h_kv, self.head_dim, self.blocks
+        at, out = 0, {}
+        for name, dtype, shape in (("codes", torch.float8_e4m3fn, (c, h, nb, 2, 64 * d)), ("scales", torch.float32, (c, h, nb, 2)),
+                                   ("k_tail", torch.float16, (c, h, 64, d)), ("v_tail", torch.float16, (c, h, d, 64)), ("tail_block", torch.int32, (c, h))):
+            n = int(np.prod(shape, dtype=np.int64)) * dtype.itemsize
+            out[name] = self.storage[at: at + n].view(dtype).view(shape)
+            at += (n + 255) // 256 * 256
+        return out
+
+
+def _offsets(what: str, *values) -> None:
+    for v in values:
+        if not 0 <= int(v) < 1 << 63:
+            raise NativeError(f"{what}: offset {v} is out of range")
+
+
+def _sizes(what: str, *values) -> None:
+    """The C interface takes 32-bit sizes: a negative or larger one would wrap around."""
+    for v in values:
+        if not 0 <= int(v) < 1 << 31:
+            raise NativeError(f"{what}: {v} is out of range")
+
+
+def _int32(what: str, values) -> np.ndarray:
+    a = np.asarray(values)
+    if a.ndim != 1 or (a.size and (a.dtype.kind not in "iu" or int(a.max()) >= 1 << 31 or int(a.min()) < -(1 << 31))):
+        raise NativeError(f"{what}: a list of whole numbers below 2^31 is needed")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _device_array(t, dtype, n, what):
+    if t is None:
+        return None
+    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or t.numel() < n:
+        raise NativeError(f"{what} must be a contiguous CUDA tensor of {n} {dtype}")
+    return t.data_ptr()
+
+
 class NativePlan:
     def __init__(self, ptr: int, owned: bool = True, keepalive=None):
         self._lib = get_lib()
         self._ptr = ptr
         self._owned = owned
         self._keepalive = keepalive
+        self._held = []          # tensors that commands of this plan point at
 
     # -- construction ------------------------------------------------------------------------------
     @classmethod
@@ -230,6 +318,66 @@ class NativePlan:
     def add_argmax(self, src_off: int, rows: int, advance: bool = False, max_seq: int = 0, name: str = "argmax") -> None:
         if self._lib.k44b_plan_add_argmax(self._ptr, name.encode(), int(src_off), int(rows), int(bool(advance)), int(max_seq)) != 0:
             raise NativeError(f"add_argmax: {last_error()}")
+
+    # -- decoder operators (no counterpart in the reference; include/k44b.h) -----------------------------------------------
+    def add_window_attn(self, q_off, k_off, v_off, out_off, h_q, h_kv, head_dim, seq_len, window=0, sinks=0, theta=10000.0, llama3=False,
+                        name="window_attn") -> None:
+        """Rotary + causal attention of every block of `seq_len` columns (any length) with a sliding window (0: none) and sinks."""
+        _offsets("add_window_attn", q_off, k_off, v_off, out_off)
+        _sizes("add_window_attn", h_q, h_kv, head_dim, seq_len, window, sinks)
+        if self._lib.k44b_plan_add_window_attn(self._ptr, name.encode(), int(q_off), int(k_off), int(v_off), int(out_off), int(h_q), int(h_kv), int(head_dim),
+                                               int(seq_len), int(window), int(sinks), float(theta), int(bool(llama3))) != 0:
+            raise NativeError(f"add_window_attn: {last_error()}")
+
+    def add_kv8_fill(self, cache: KV8Cache, k_off, v_off, seq_len, theta=10000.0, llama3=False, name="kv8_fill") -> None:
+        """Keys (not yet rotated) and values of a prompt plan into an 8-bit cache; see `set_sequences`."""
+        _offsets("add_kv8_fill", k_off, v_off)
+        _sizes("add_kv8_fill", seq_len)
+        if self._lib.k44b_plan_add_kv8_fill(self._ptr, name.encode(), ctypes.byref(cache._desc), int(k_off), int(v_off), int(seq_len), float(theta),
+                                            int(bool(llama3))) != 0:
+            raise NativeError(f"add_kv8_fill: {last_error()}")
+        self._held.append(cache)
+
+    def add_kv8_attn(self, cache: KV8Cache, q_off, k_off, v_off, out_off, h_q, window=0, sinks=0, theta=10000.0, llama3=False, name="kv8_attn") -> None:
+        """One new token per column, each at its own position (`set_positions`), appended to the cache and attending to it."""
+        _offsets("add_kv8_attn", q_off, k_off, v_off, out_off)
+        _sizes("add_kv8_attn", h_q, window, sinks)
+        if self._lib.k44b_plan_add_kv8_attn(self._ptr, name.encode(), ctypes.byref(cache._desc), int(q_off), int(k_off), int(v_off), int(out_off), int(h_q),
+                                            int(window), int(sinks), float(theta), int(bool(llama3))) != 0:
+            raise NativeError(f"add_kv8_attn: {last_error()}")
+        self._held.append(cache)
+
+    def add_logprobs(self, src_off, rows, targets=None, logprobs=None, entropy=None, top_rows=None, top_logprobs=None, name="logprobs") -> None:
+        """Per column of a logits tensor: log probability of row targets[column], entropy (nats), and the most probable rows with their
+        log probabilities ([top, columns] tensors; `top` is their first size). All are CUDA tensors: int32 for rows, float32 for the rest."""
+        import torch
+        _offsets("add_logprobs", src_off)
+        _sizes("add_logprobs", rows)
+        cols = int(self._lib.k44b_plan_columns(self._ptr))
+        top = 0 if top_rows is None else int(top_rows.shape[0])
+        if top and (top_rows.numel() != top * cols or top_logprobs is None or tuple(top_logprobs.shape) != tuple(top_rows.shape)):
+            raise NativeError("add_logprobs: top_rows and top_logprobs must be [top, columns]")
+        f32, i32 = torch.float32, torch.int32
+        p = [_device_array(targets, i32, cols, "targets"), _device_array(logprobs, f32, cols, "logprobs"), _device_array(entropy, f32, cols, "entropy"),
+             _device_array(top_rows, i32, top * cols, "top_rows"), _device_array(top_logprobs, f32, top * cols, "top_logprobs")]
+        if self._lib.k44b_plan_add_logprobs(self._ptr, name.encode(), int(src_off), int(rows), p[0], p[1], p[2], top, p[3] if top else None, p[4] if top else None) != 0:
+            raise NativeError(f"add_logprobs: {last_error()}")
+        self._held.append((targets, logprobs, entropy, top_rows, top_logprobs))
+
+    def set_positions(self, positions, stream=None) -> None:
+        """Position of the new token of the first columns (-1: idle) for `add_kv8_attn`."""
+        t = _int32("set_positions", positions)
+        if self._lib.k44b_plan_set_positions(self._ptr, t.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), int(t.size), ctypes.c_void_p(self._stream_ptr(stream))) != 0:
+            raise NativeError(f"set_positions: {last_error()}")
+
+    def set_sequences(self, cache_columns, lengths, stream=None) -> None:
+        """For `add_kv8_fill`: the cache column of each sequence (-1: nowhere) and its length."""
+        c, n = _int32("set_sequences", cache_columns), _int32("set_sequences", lengths)
+        if c.size != n.size:
+            raise NativeError("set_sequences: one cache column and one length per sequence")
+        i32p = ctypes.POINTER(ctypes.c_int32)
+        if self._lib.k44b_plan_set_sequences(self._ptr, c.ctypes.data_as(i32p), n.ctypes.data_as(i32p), int(c.size), ctypes.c_void_p(self._stream_ptr(stream))) != 0:
+            raise NativeError(f"set_sequences: {last_error()}")
 
     # -- 2-D image planes -------------------------------------------------------------------------------------------------
     IMAGE_OPS = {"maxpool2": 7, "maxpool5": 8, "upsample2": 9, "space_to_depth": 10, "upconv_scatter": 11, "halo_clear": 12}
