@@ -61,14 +61,17 @@ struct Kv8AttnArgs {
     const int *positions = nullptr;                  // per column: position of its new token, -1 idle
     const float2 *rope = nullptr;
     uint32_t *status = nullptr;
+    uint4 *q_frag = nullptr;                         // [column][head]: the group's rotated q as operand words
     float *partial = nullptr;                        // [worker][2][8 or 16 heads][head_dim + 2]
     uint32_t *counters = nullptr;                    // [column][head], zero between launches
     uint32_t pitch = 0, columns = 0, h_q = 0, window = 0, sinks = 0;
+    uint32_t workers = 0, spread = 1;                // warps, and their step over the shares (set by the launcher)
     unsigned long long wait_cycles = 0;
 };
 constexpr uint32_t kKv8MaxColumns = 4096;
 cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, uint32_t num_sms, bool pdl, cudaStream_t s);
 cudaError_t kv8_attn_setup();                        // opt in to large dynamic shared memory (once per device)
+uint64_t kv8_attn_frag_bytes(uint32_t columns, uint32_t h_kv, uint32_t group, uint32_t head_dim);
 uint64_t kv8_attn_partial_bytes(uint32_t num_sms, uint32_t group, uint32_t head_dim);
 
 // ---- prompt attention with a window and sinks ---------------------------------------------------------------------------

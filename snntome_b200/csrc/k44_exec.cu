@@ -224,6 +224,7 @@ void Executor::release() {
     cudaFree(d_window_); d_window_ = nullptr; window_bytes_ = 0;
     cudaFree(d_kv8_partial_); d_kv8_partial_ = nullptr; kv8_partial_bytes_ = 0;
     cudaFree(d_kv8_counters_); d_kv8_counters_ = nullptr; kv8_counter_bytes_ = 0;
+    cudaFree(d_kv8_frag_); d_kv8_frag_ = nullptr; kv8_frag_bytes_ = 0;
     cudaFree(d_logprob_); d_logprob_ = nullptr; logprob_bytes_ = 0;
     cudaFree(d_sync_); d_sync_ = nullptr;
     cudaFree(d_peers_); d_peers_ = nullptr;
@@ -658,7 +659,7 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         if (w.h_q / w.h_kv > 16u) return bad("at most 16 query heads per key / value head");
         if (w.cache_columns < columns_) return bad("the cache has fewer columns than the plan");
         if (columns_ > kKv8MaxColumns) return bad("at most " + std::to_string(kKv8MaxColumns) + " columns");
-        if ((uint64_t)columns_ * w.h_kv * (cache.blocks + 1ull) >= 0xffffffffull) return bad("the cache is too large");
+        if ((uint64_t)columns_ * w.h_kv * (cache.blocks + 8ull) >= 0xffffffffull) return bad("the cache is too large");
         Kv8AttnArgs &a = dw.kv8;
         a.cache = cache; a.q = canvas_ + w.src_off; a.k = canvas_ + w.src2_off; a.v = canvas_ + w.src3_off; a.out = canvas_ + w.y_off;
         a.pitch = pitch_; a.columns = columns_; a.h_q = w.h_q; a.window = w.window; a.sinks = w.sinks; a.status = d_status_; a.wait_cycles = wait_cycles;
@@ -666,9 +667,10 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, w.max_seq))) return false;
         if (!check(kv8_attn_setup(), "kernel attribute setup")) return false;
         if (!reserve(d_kv8_partial_, kv8_partial_bytes_, kv8_attn_partial_bytes((uint32_t)num_sms_, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") ||
+            !reserve(d_kv8_frag_, kv8_frag_bytes_, kv8_attn_frag_bytes(columns_, w.h_kv, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") ||
             !reserve(d_kv8_counters_, kv8_counter_bytes_, (uint64_t)columns_ * w.h_kv * sizeof(uint32_t), "attention scratch allocation")) return false;
-        a.partial = (float *)d_kv8_partial_; a.counters = (uint32_t *)d_kv8_counters_;
-        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_KV8_ATTN) { o.kv8.partial = a.partial; o.kv8.counters = a.counters; }
+        a.partial = (float *)d_kv8_partial_; a.counters = (uint32_t *)d_kv8_counters_; a.q_frag = (uint4 *)d_kv8_frag_;
+        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_KV8_ATTN) { o.kv8.partial = a.partial; o.kv8.counters = a.counters; o.kv8.q_frag = a.q_frag; }
         return true;
     }
     case AUX_LOGPROBS: {
@@ -1205,7 +1207,7 @@ bool Executor::launch_one(DeviceWave &w, cudaStream_t stream, uint32_t peer_slac
         switch (w.aux.kind) {
         case AUX_WINDOW_ATTN: launches_ += 2u; return check(launch_window_attn(w.window, w.window_maps, pdl_, stream), what.c_str());
         case AUX_KV8_FILL: ++launches_; return check(launch_kv8_fill(w.fill, pdl_, stream), what.c_str());
-        case AUX_KV8_ATTN: ++launches_; return check(launch_kv8_attn(w.kv8, (uint32_t)num_sms_, pdl_, stream), what.c_str());
+        case AUX_KV8_ATTN: launches_ += 2u; return check(launch_kv8_attn(w.kv8, (uint32_t)num_sms_, pdl_, stream), what.c_str());
         case AUX_LOGPROBS: launches_ += 2u; return check(launch_logprobs(w.logprob, pdl_, stream), what.c_str());
         default: break;
         }

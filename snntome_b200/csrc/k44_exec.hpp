@@ -178,8 +178,8 @@ class Executor {
     int *d_positions_ = nullptr;
     int2 *d_sequences_ = nullptr;
     std::vector<int32_t> h_slots_, h_lengths_;      // what set_sequences was given last
-    void *d_window_ = nullptr, *d_kv8_partial_ = nullptr, *d_kv8_counters_ = nullptr, *d_logprob_ = nullptr;
-    uint64_t window_bytes_ = 0, kv8_partial_bytes_ = 0, kv8_counter_bytes_ = 0, logprob_bytes_ = 0;
+    void *d_window_ = nullptr, *d_kv8_partial_ = nullptr, *d_kv8_counters_ = nullptr, *d_kv8_frag_ = nullptr, *d_logprob_ = nullptr;
+    uint64_t window_bytes_ = 0, kv8_partial_bytes_ = 0, kv8_counter_bytes_ = 0, kv8_frag_bytes_ = 0, logprob_bytes_ = 0;
     // neuron sharding over several GPUs (see PeerArgs)
     uint32_t *d_sync_ = nullptr;          // kSyncWords words, allocated on first use
     PeerArgs *d_peers_ = nullptr;

@@ -7,6 +7,8 @@
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
 
+#include <numeric>
+
 namespace k44b {
 namespace {
 
@@ -163,34 +165,46 @@ __global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a) 
 // o = sum_t softmax_t(q . k_t / sqrt(D)) v_t over the visible positions t of a column, for the group of query heads that share
 // one key / value head, so that every code is read once. Memory-bound: 2 D bytes per position and key / value head.
 //
-// Work: a unit is one visible 8-bit block of one (column, head), or its open block with the new token. All units in a row
-// (column, head, block) are cut into equal shares, one per warp of the grid, whatever the columns' lengths; a warp that holds
-// a (column, head) whole writes its output, the others leave (accumulator, maximum, sum) and the last one to arrive adds the
-// parts in the order of the warps, so that the result does not depend on the order of arrival.
-// Loads: a block is 2 * 64 * D contiguous bytes; each warp keeps a ring of them in flight with bulk copies.
+// Two launches. The first rotates q and k, leaves q in the order in which the second loads it, appends the new tokens to the open
+// blocks and brings completed blocks to 8 bits: on the canvas a column's channels are `pitch` elements apart, and warps that each
+// gather theirs cost 6 to 8 us of a step of 64 columns (11 000 to 16 000 cycles per warp, 32 sectors per load), a transposing
+// pass over 8 columns at a time 2 to 3.
+//
+// Work of the second: a unit is one visible 8-bit block of one (column, head), or its open block. All units in a row
+// (column, head, block), each with a weight, are cut into equal shares, one per warp of the grid, whatever the columns' lengths; a
+// warp that holds a (column, head) whole writes its output, the others leave (accumulator, maximum, sum) and the last one to
+// arrive adds the parts in the order of the warps, so that the result does not depend on the order of arrival.
+// Loads: each warp keeps a ring of granules of 64 * D bytes in flight with bulk copies: the keys of an 8-bit block are one
+// granule, its values another, the FP16 keys of the open block two, its values two. Nothing in the walk over the blocks waits for
+// a global load of its own; scales are fetched 32 blocks at a time.
 // Products on mma.sync: 8 (or 16) query heads are the rows of m16n8k16 — tcgen05 would need 64 rows and its operands as FP16
 // in shared memory, for a kernel that waits for HBM. Keys: a lane takes 16 consecutive dimensions of one token (16 bytes),
 // values: 16 consecutive tokens of one dimension; which logical k index they stand for is free as long as the other operand
 // agrees, so codes go from shared memory to the operand registers without a shuffle: token of score tile i, column 2 j + e =
 // 16 j + 2 i + e, and the scores' accumulator layout is the second product's A operand as it stands.
 // The values' scale is folded into the exponent (p' = p * scale): p' <= 1 is what is rounded to FP16, and the sum uses p' / scale.
-// q is split into two FP16 numbers (high and low part): with exact codes the scores are then as good as in 32 bits.
-constexpr uint32_t kWarps64 = 8, kWarps128 = 4, kStages = 3;
+// q is split into two FP16 numbers (high and low part): with exact codes the scores are then as good as in 32 bits. With up to 8
+// heads the low parts are rows 8 to 15 of the operand, which would be empty, and cost nothing.
+constexpr uint32_t kOpenWeight = 4;                              // an open block: one and a half times the bytes, and the work around it
+// warps per SM and granules per warp (192 KB of an SM's shared memory in all): as many warps as the registers allow
+template <int D, bool WIDE> constexpr uint32_t kWarps = WIDE || D == 128 ? 8u : 12u;
+template <int D, bool WIDE> constexpr uint32_t kRing = 192u * 1024u / (kWarps<D, WIDE> * kKv8Block * D);
 
 __device__ __forceinline__ void mma16816(float &c0, float &c1, float &c2, float &c3, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // what a column's token sees: 8-bit blocks [0, sink_blocks) and [from, open), and the open block
 struct Seen {
-    uint32_t sink_blocks, from, open, units;
+    uint32_t sink_blocks, from, open, units;            // units: those 8-bit blocks and the open one
+    __device__ uint32_t weight() const { return units - 1u + kOpenWeight; }
 };
 __device__ __forceinline__ Seen seen_of(int pos, uint32_t window, uint32_t sinks) {
     Seen s;
@@ -204,31 +218,165 @@ __device__ __forceinline__ Seen seen_of(int pos, uint32_t window, uint32_t sinks
     return s;
 }
 
-template <int D, int WARPS, bool WIDE>           // WIDE: 9 to 16 query heads per key / value head
-__global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8AttnArgs a) {
-    constexpr int DT = D / 8, KS = D / 16, HF = D / 64, R = WIDE ? 2 : 1;      // dimension tiles, k steps, halves, row sets
-    constexpr uint32_t BLK = 2u * kKv8Block * D, GP = 8u * R, PROW = D + 2u;
+// A column's position where it is inside the cache, -1 (idle) otherwise.
+__device__ __forceinline__ int position_of(const Kv8AttnArgs &a, uint32_t c) {
+    const int p = a.positions[c];
+    return p >= 0 && (uint32_t)p < a.cache.max_seq ? p : -1;
+}
+
+// First launch. Grid (8 columns, key / value head, role): role 0 q, 1 keys, 2 values, a warp per column. It lets the second launch start
+// once its own predecessors are done: what that one does before it waits in turn (cutting up the work, copies of 8-bit blocks) needs
+// nothing of this one's, so the two overlap.
+// Roles 1 and 2 read a block that is about to be complete before they wait for the new token's row, and patch that in.
+template <int D, bool WIDE>           // WIDE: 9 to 16 query heads per key / value head
+__global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs a) {
+    constexpr int KS = D / 16, HF = D / 64, R = WIDE ? 2 : 1, TILE = kKv8Block * D, ROWS = 8 * R * D, PAD = ROWS + 8;
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[WARPS * kStages];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, j = lane & 3u;
+    const uint32_t H = a.cache.h_kv, G = a.h_q / H, C = a.columns;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // ---- rows of the head for 8 columns, turned: [column][row] ----
+    __half *xs = reinterpret_cast<__half *>(smem_raw);
+    const uint32_t head = blockIdx.y, c0 = blockIdx.x * 8u, col = c0 + warp;
+    const bool is_q = blockIdx.z == 0u, is_k = blockIdx.z == 1u;
+    const int pos = col < C ? position_of(a, col) : -1;
+    const uint64_t ch = (uint64_t)col * H + head;
+    const uint32_t b = (uint32_t)pos / kKv8Block, slot = (uint32_t)pos % kKv8Block;
+    constexpr int N = TILE / 8 / 32;                                           // 16-byte pieces of a block per lane
+    __half *tail = (is_k ? a.cache.k_tail : a.cache.v_tail) + ch * TILE;
+    uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + b) * (2u * TILE) + (is_k ? 0u : TILE);
+    uint4 piece[N];
+    const bool whole = !is_q && pos >= 0 && slot == kKv8Block - 1u;
+    int tag = 0;
+    if (!is_q && pos >= 0) tag = a.cache.tail_block[ch];
+    if (whole)
+#pragma unroll
+        for (int i = 0; i < N; ++i) piece[i] = reinterpret_cast<const uint4 *>(tail)[32 * i + lane];
+    const uint32_t rows = is_q ? G * D : (uint32_t)D;
+    const __half *rows_of = is_q ? a.q + (uint64_t)head * G * D * a.pitch : (is_k ? a.k : a.v) + (uint64_t)head * D * a.pitch;
+    for (uint32_t r = tid; r < rows; r += 256u) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(rows_of + (uint64_t)r * a.pitch + c0));
+        const __half *h = reinterpret_cast<const __half *>(&v);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) xs[c * PAD + r] = h[c];
+    }
+    if (is_q) for (uint32_t r = rows + tid; r < (uint32_t)ROWS; r += 256u)      // rows of the operand without a head
+#pragma unroll
+        for (int c = 0; c < 8; ++c) xs[c * PAD + r] = __half(0.f);
+    if (is_q && head == 0u && lane == 0u && col < C && pos < 0 && a.positions[col] >= 0) atomicOr(a.status, (uint32_t)ST_BAD_INDEX);
+    __syncthreads();
+    if (pos < 0) return;
+    const float2 *cs = a.rope + (uint64_t)pos * (D / 2);
+    __half *x = xs + warp * PAD;
+    if (is_q) {
+        // ---- operand words of lane (g, j): row g (+ 8), dimensions 64 f + 16 j + 4 s + 2 t, + 1; high parts, then low parts ----
+        uint4 *frag = a.q_frag + ch * (R * KS * 32u) + lane;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int f = 0; f < HF; ++f) {
+                const uint32_t d0 = 64u * f + 16u * j, p0 = d0 % (D / 2);
+                const __half *lo16 = x + (g + 8u * r) * D + p0;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float y[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int i = 4 * s + 2 * t + e;
+                            float u = __half2float(lo16[i]), v = __half2float(lo16[i + D / 2]);
+                            rotate(u, v, __ldg(cs + p0 + i));
+                            y[e] = d0 < D / 2 ? u : v;
+                        }
+                        hi[t] = pack2(y[0], y[1]);
+                        const float2 hf = half2_of(hi[t]);
+                        lo[t] = pack2(y[0] - hf.x, y[1] - hf.y);
+                    }
+                    frag[(r * KS + 4 * f + s) * 32] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+                }
+            }
+        }
+        return;
+    }
+    // ---- append the new token to the open block (whose number the second launch writes down) ----
+    const bool rebuild = tag != (int)b && slot != 0u;                          // back inside a block that was complete: its rows start from its 8 bits
+    if (rebuild) {
+        const float2 both = a.cache.scales[ch * a.cache.blocks + b];
+        const float old = is_k ? both.x : both.y;
+        for (uint32_t e = lane; e < TILE / 2u; e += 32u) {
+            const uint32_t c2 = 2u * e, t = (c2 >> 6) & 63u, d = (c2 >> 12) * 64u + (c2 & 63u);
+            const float2 f = half2_of(from_codes(*reinterpret_cast<const uint16_t *>(codes + c2)));
+            const uint32_t v = pack2(f.x * old, f.y * old);
+            if (!is_k) *reinterpret_cast<uint32_t *>(tail + c2) = v;
+            else if (t < slot) *reinterpret_cast<uint32_t *>(tail + t * D + d) = v;
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int f = 0; f < HF; ++f) {
+        const uint32_t p = 32u * f + lane;
+        if (is_k) {
+            float u = __half2float(x[p]), v = __half2float(x[p + D / 2]);
+            rotate(u, v, __ldg(cs + p));
+            const __half hu = __float2half_rn(u), hv = __float2half_rn(v);
+            tail[slot * D + p] = hu; tail[slot * D + p + D / 2] = hv;
+            x[p] = hu; x[p + D / 2] = hv;
+        } else {
+            tail[p * 64u + slot] = x[p];
+            tail[(p + D / 2) * 64u + slot] = x[p + D / 2];
+        }
+    }
+    if (!whole) return;
+    // ---- the block is complete: bring it to 8 bits ----
+    __syncwarp();
+    if (rebuild)
+#pragma unroll
+        for (int i = 0; i < N; ++i) piece[i] = reinterpret_cast<const uint4 *>(tail)[32 * i + lane];
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {                                              // the new token's row (keys) or column (values)
+        const uint32_t at = (32u * i + lane) * 8u;
+        if (is_k) { if (at / D == kKv8Block - 1u) piece[i] = *reinterpret_cast<const uint4 *>(x + at % D); }
+        else if ((at & 63u) == 56u) piece[i].w = (piece[i].w & 0xffffu) | ((uint32_t)__half_as_ushort(x[at >> 6]) << 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { const float2 f = half2_of(word(piece[i], e)); mx = amax_of(amax_of(mx, f.x), f.y); }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float scale = scale_of(mx), inv = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float2 x0 = half2_of(piece[i].x), x1 = half2_of(piece[i].y), x2 = half2_of(piece[i].z), x3 = half2_of(piece[i].w);
+        const uint32_t at = (32u * i + lane) * 8u, t = at / D, d = at % D;
+        *reinterpret_cast<uint2 *>(codes + (is_k ? (d >> 6) * 4096u + t * 64u + (d & 63u) : at)) = make_uint2(codes4(x0.x, x0.y, x1.x, x1.y, inv), codes4(x2.x, x2.y, x3.x, x3.y, inv));
+    }
+    if (lane == 0u) reinterpret_cast<float *>(a.cache.scales + ch * a.cache.blocks + b)[is_k ? 0 : 1] = scale;
+}
+
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(const Kv8AttnArgs a) {
+    constexpr int DT = D / 8, KS = D / 16, HF = D / 64, R = WIDE ? 2 : 1;      // dimension tiles, k steps, halves, row sets
+    constexpr uint32_t GRAN = kKv8Block * D, WARPS = kWarps<D, WIDE>, RING = kRing<D, WIDE>, GP = 8u * R, PROW = D + 2u;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[WARPS * RING];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, j = lane & 3u;
     const uint32_t H = a.cache.h_kv, G = a.h_q / H, C = a.columns;
-    uint32_t *prefix = reinterpret_cast<uint32_t *>(smem_raw + WARPS * kStages * BLK);      // [C + 1] units before a column
-    const uint32_t ring = ptx::smem_addr(smem_raw) + warp * kStages * BLK;
-    const uint32_t bar0 = ptx::smem_addr(bars) + warp * kStages * 8u;
+    uint8_t *const ring_ptr = smem_raw + warp * RING * GRAN;
+    const uint32_t ring = ptx::smem_addr(ring_ptr);
+    const uint32_t bar0 = ptx::smem_addr(bars) + warp * RING * 8u;
     if (lane == 0u) {
-        for (uint32_t s = 0; s < kStages; ++s) ptx::mbar_init(bar0 + 8u * s, 1);
+        for (uint32_t s = 0; s < RING; ++s) ptx::mbar_init(bar0 + 8u * s, 1);
         ptx::fence_mbar_init();
     }
-    dep_enter();
-    // ---- units before each column ----
-    auto pos_of = [&](uint32_t c) -> int {
-        const int p = a.positions[c];
-        return p >= 0 && (uint32_t)p < a.cache.max_seq ? p : -1;
-    };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // ---- cut up the work: weight before each column ----
+    uint32_t *prefix = reinterpret_cast<uint32_t *>(smem_raw + WARPS * RING * GRAN);       // [C + 1]
     for (uint32_t c = threadIdx.x; c < C; c += WARPS * 32u) {
-        const int p = pos_of(c);
-        if (p < 0 && a.positions[c] >= 0 && blockIdx.x == 0u) atomicOr(a.status, (uint32_t)ST_BAD_INDEX);
-        prefix[c + 1u] = H * (p < 0 ? 1u : seen_of(p, a.window, a.sinks).units);
+        const int p = position_of(a, c);
+        prefix[c + 1u] = H * (p < 0 ? 1u : seen_of(p, a.window, a.sinks).weight());
     }
     __syncthreads();
     if (warp == 0u) {
@@ -243,107 +391,147 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
         if (lane == 0u) prefix[0] = 0u;
     }
     __syncthreads();
-    const uint32_t total = prefix[C];
-    const uint32_t workers = min(gridDim.x * WARPS, total), me = warp * gridDim.x + blockIdx.x;       // neighbours sit on different SMs
+    // Which share a warp takes: its number times a step that shares no factor with the number of warps. Shares that cost more than
+    // they weigh (open blocks) come at a regular distance; in the order of the warps they would meet on the same few SMs where that
+    // distance divides the SMs (64 columns x 8 heads did), with a step near the golden ratio an SM's shares lie all over the row.
+    const uint32_t me = (blockIdx.x * WARPS + warp) * a.spread % a.workers, total = prefix[C];
+    const uint32_t workers = min(a.workers, total), each = total / workers, more = total % workers;       // the first `more` shares weigh one more
     if (me >= workers) return;
-    auto share = [&](uint32_t w) -> uint32_t { return (uint32_t)((uint64_t)w * total / workers); };
-    auto worker_of = [&](uint32_t u) -> uint32_t { return (uint32_t)((((uint64_t)u + 1u) * workers - 1u) / total); };
-    const uint32_t u_begin = share(me), u_end = share(me + 1u);
-    uint32_t col = 0;                                                        // the column that holds u_begin
+    auto share = [&](uint32_t w) -> uint32_t { return w * each + min(w, more); };
+    auto worker_of = [&](uint32_t x) -> uint32_t { return x < more * (each + 1u) ? x / (each + 1u) : more + (x - more * (each + 1u)) / each; };
+    const uint32_t x_begin = share(me), x_end = share(me + 1u);             // this warp's units are those that start in here
+    // a place in the row of units
+    struct At {
+        uint32_t col, head, unit, x;                                        // x: where the unit starts
+        int pos;
+        Seen seen;
+    };
+    auto enter = [&](At &t) {
+        t.pos = position_of(a, t.col);
+        t.seen = t.pos < 0 ? Seen{0u, 0u, 0u, 1u} : seen_of(t.pos, a.window, a.sinks);
+    };
+    auto per_head = [&](const At &t) -> uint32_t { return t.pos < 0 ? 1u : t.seen.weight(); };
+    auto next_head = [&](At &t) {                                           // to the first unit of the next (column, head)
+        t.x += per_head(t) - t.unit;
+        t.unit = 0u;
+        if (++t.head == H) { t.head = 0u; ++t.col; if (t.col < C) enter(t); }
+    };
+    auto block_of = [&](const Seen &s, uint32_t unit) -> uint32_t { return unit < s.sink_blocks ? unit : s.from + (unit - s.sink_blocks); };
+    At at;
     {
         uint32_t lo = 0, hi = C - 1u;
-        while (lo < hi) { const uint32_t mid = (lo + hi + 1u) >> 1; if (prefix[mid] <= u_begin) lo = mid; else hi = mid - 1u; }
-        col = lo;
+        while (lo < hi) { const uint32_t mid = (lo + hi + 1u) >> 1; if (prefix[mid] <= x_begin) lo = mid; else hi = mid - 1u; }
+        at.col = lo;
+        enter(at);
+        const uint32_t rem = x_begin - prefix[lo], per = per_head(at);
+        at.head = rem / per; at.unit = rem % per; at.x = x_begin;
     }
-    // ---- the ring's own walk over this warp's 8-bit blocks, ahead of the one below ----
-    uint32_t iu = u_begin, icol = col, ihead = 0, iper = 1, iat = 0, issued = 0;
-    Seen iseen = {};
-    int ipos = -1;
-    auto enter_issue = [&]() {
-        ipos = pos_of(icol);
-        iseen = ipos < 0 ? Seen{0u, 0u, 0u, 1u} : seen_of(ipos, a.window, a.sinks);
-        iper = iseen.units;
-    };
-    enter_issue();
-    { const uint32_t rem = iu - prefix[icol]; ihead = rem / iper; iat = rem % iper; }
-    const uint64_t policy = ptx::policy_evict_first();
-    auto issue_next = [&]() {                                                 // lane 0 only; next 8-bit block into the next stage
-        while (iu < u_end) {
-            const bool block8 = iat + 1u < iper;
-            const uint32_t b = iat < iseen.sink_blocks ? iat : iseen.from + (iat - iseen.sink_blocks);
-            const uint64_t ch = (uint64_t)icol * H + ihead;
-            ++iu; ++iat;
-            const bool wrap = iat == iper;
-            if (block8) {
-                const uint32_t st = issued % kStages;
-                ptx::mbar_arrive_expect_tx(bar0 + 8u * st, BLK);
-                ptx::bulk_g2s(ring + st * BLK, a.cache.codes + (ch * a.cache.blocks + b) * BLK, BLK, bar0 + 8u * st, policy);
-                ++issued;
-            }
-            if (wrap) {
-                iat = 0;
-                if (++ihead == H) { ihead = 0; ++icol; if (iu < u_end) enter_issue(); }
-            }
-            if (block8) return;
+    if (at.unit >= at.seen.units) next_head(at);                            // the share begins inside an open block's weight
+    // ---- q of a (column, head) as operands, and the scales of 32 of its blocks: a lane holds those of one ----
+    const float sm = rsqrtf((float)D) * kLog2e;
+    uint32_t qh[R][KS][2], ql[R][KS][2];
+    float sc_mul = 0.f, sc_log = 0.f, sc_inv = 0.f;
+    auto fetch_scales = [&](uint32_t first) {
+        const uint32_t unit = first + lane;
+        if (at.pos >= 0 && unit + 1u < at.seen.units) {
+            const float2 sc = __ldg(a.cache.scales + ((uint64_t)at.col * H + at.head) * a.cache.blocks + block_of(at.seen, unit));
+            sc_mul = sc.x * sm; sc_log = log2f(sc.y); sc_inv = 1.0f / sc.y;
         }
     };
+    auto fetch_head = [&]() {
+        const uint4 *frag = a.q_frag + ((uint64_t)at.col * H + at.head) * (R * KS * 32u) + lane;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const uint4 w = __ldg(frag + (r * KS + k) * 32);
+                qh[r][k][0] = w.x; qh[r][k][1] = w.y; ql[r][k][0] = w.z; ql[r][k][1] = w.w;
+            }
+        fetch_scales(at.unit);
+    };
+    // ---- the ring's own walk, one granule per call, lane 0 only: runs of contiguous granules ----
+    At ahead = at;
+    uint32_t issued = 0, left = 0, rem = 0;                                  // granules left in the run, bytes left in it
+    bool values = false;                                                     // the open block's keys are out, its values are next
+    const uint8_t *src = nullptr;
+    const uint64_t policy = ptx::policy_evict_first();
+    bool early = true;                                                       // the first launch may still be at work: only what was there before it
+    auto next_run = [&]() -> bool {
+        while (ahead.x < x_end && ahead.col < C) {
+            if (ahead.pos < 0) { next_head(ahead); continue; }
+            if (early && ahead.unit + 1u >= ahead.seen.units) return false;
+            const Seen &n = ahead.seen;
+            const uint64_t ch = (uint64_t)ahead.col * H + ahead.head;
+            if (ahead.unit + 1u < n.units) {
+                const uint32_t run = min(min((ahead.unit < n.sink_blocks ? n.sink_blocks : n.units - 1u) - ahead.unit, x_end - ahead.x), 65536u);
+                src = a.cache.codes + (ch * a.cache.blocks + block_of(n, ahead.unit)) * (2u * GRAN);
+                left = 2u * run; rem = left * GRAN;
+                ahead.unit += run; ahead.x += run;
+            } else if (!values) {                                            // only the rows that are there
+                src = reinterpret_cast<const uint8_t *>(a.cache.k_tail) + ch * (2u * GRAN);
+                left = 2u; rem = ((uint32_t)ahead.pos % kKv8Block + 1u) * (2u * D);
+                values = true;
+            } else {
+                src = reinterpret_cast<const uint8_t *>(a.cache.v_tail) + ch * (2u * GRAN);
+                left = 2u; rem = 2u * GRAN;
+                values = false;
+                next_head(ahead);
+            }
+            return true;
+        }
+        return false;
+    };
+    auto issue = [&]() {
+        if (left == 0u && !next_run()) return;
+        const uint32_t bar = bar0 + 8u * (issued % RING), bytes = min(rem, GRAN);
+        if (bytes) {
+            ptx::mbar_arrive_expect_tx(bar, bytes);
+            ptx::bulk_g2s(ring + issued % RING * GRAN, src, bytes, bar, policy);
+        } else ptx::mbar_arrive(bar);
+        src += bytes; rem -= bytes;
+        --left; ++issued;
+    };
     if (lane == 0u)
-        for (uint32_t s = 0; s < kStages; ++s) issue_next();
+        for (uint32_t s = 0; s < RING; ++s) issue();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    early = false;
+    if (lane == 0u)
+        while (issued < RING && (left || next_run())) issue();
     __syncwarp();
+    if (at.x < x_end && at.col < C) fetch_head();
 
-    const float sm = rsqrtf((float)D) * kLog2e;
-    uint32_t u = u_begin, consumed = 0;
+    uint32_t consumed = 0;
     bool ok = true;
-    while (u < u_end && ok) {
-        while (prefix[col + 1u] <= u) ++col;
-        const int pos = pos_of(col);
-        const Seen sn = pos < 0 ? Seen{0u, 0u, 0u, 1u} : seen_of(pos, a.window, a.sinks);
-        const uint32_t rem = u - prefix[col], head = rem / sn.units, at0 = rem % sn.units;
-        const uint32_t n_units = min(sn.units - at0, u_end - u);               // this warp's part of the (column, head)
-        const uint32_t seg0 = prefix[col] + head * sn.units;
+    auto granule = [&](uint32_t i) -> uint8_t * { return ring_ptr + ((consumed + i) % RING) * GRAN; };
+    auto arrived = [&](uint32_t i) -> bool {                                  // whole warp; bounded
+        const uint32_t n = consumed + i, bar = bar0 + 8u * (n % RING), ph = (n / RING) & 1u;
+        bool here = ptx::mbar_try_wait(bar, ph);
+        if (!here) {
+            const long long t0 = clock64();
+            while (!(here = ptx::mbar_try_wait(bar, ph)) && (unsigned long long)(clock64() - t0) < a.wait_cycles) {}
+        }
+        return __all_sync(0xffffffffu, here ? 1 : 0) != 0;
+    };
+    auto release = [&](uint32_t n) {                                          // n granules have been read by every lane
+        __syncwarp();
+        consumed += n;
+        if (lane == 0u) for (uint32_t i = 0; i < n; ++i) issue();
+    };
+
+    for (bool first = true; at.x < x_end && at.col < C && ok; first = false) {
+        const uint32_t col = at.col, head = at.head;
+        const int pos = at.pos;
+        const Seen sn = at.seen;
         const uint64_t ch = (uint64_t)col * H + head;
         if (pos < 0) {                                                          // idle column: zeros
             for (uint32_t e = lane; e < G * D; e += 32u) a.out[((uint64_t)head * G * D + e) * a.pitch + col] = __half(0.f);
-            u += 1u;
+            next_head(at);
             continue;
         }
-        // ---- q of the group, rotated, as two FP16 operands ----
-        uint32_t qh[R][KS][2], ql[R][KS][2];
-        const float2 *cs = a.rope + (uint64_t)pos * (D / 2);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint32_t row = g + 8u * r;
-            float x[HF][16];
-#pragma unroll
-            for (int f = 0; f < HF; ++f)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    x[f][e] = row < G ? __half2float(a.q[((uint64_t)(head * G + row) * D + 64u * f + 16u * j + e) * a.pitch + col]) : 0.f;
-            if (HF == 2) {                                                      // pairs (d, d + 64): both halves of this lane
-#pragma unroll
-                for (int e = 0; e < 16; ++e) rotate(x[0][e], x[HF - 1][e], __ldg(cs + 16u * j + e));
-            } else {                                                            // pairs (d, d + 32): lane j and lane j ^ 2
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float other = __shfl_xor_sync(0xffffffffu, x[0][e], 2);
-                    float lo = j < 2u ? x[0][e] : other, hi = j < 2u ? other : x[0][e];
-                    rotate(lo, hi, __ldg(cs + 16u * (j & 1u) + e));
-                    x[0][e] = j < 2u ? lo : hi;
-                }
-            }
-#pragma unroll
-            for (int f = 0; f < HF; ++f)
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const float x0 = x[f][4 * s + 2 * t], x1 = x[f][4 * s + 2 * t + 1];
-                        const uint32_t hi = pack2(x0, x1);
-                        const float2 hf = half2_of(hi);
-                        qh[r][4 * f + s][t] = hi;
-                        ql[r][4 * f + s][t] = pack2(x0 - hf.x, x1 - hf.y);
-                    }
-        }
+        if (!first) fetch_head();
+        const uint32_t seg0 = at.x - at.unit, unit0 = at.unit;
+        const uint32_t n_units = min(sn.units - unit0, x_end - at.x);            // this warp's part of the (column, head): units start one after the other
+        const bool has_open = unit0 + n_units == sn.units;
         float acc[DT][2 * R], m[R], l[R];
 #pragma unroll
         for (int t = 0; t < DT; ++t)
@@ -352,9 +540,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
 #pragma unroll
         for (int r = 0; r < R; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
 
+        // scores of 8 tokens more: k step 4 f + t of tile i
+        auto score = [&](float (&c)[4], int k, uint32_t b0, uint32_t b1) {
+            if (WIDE) {
+                mma16816(c[0], c[1], c[2], c[3], qh[0][k][0], qh[R - 1][k][0], qh[0][k][1], qh[R - 1][k][1], b0, b1);
+                mma16816(c[0], c[1], c[2], c[3], ql[0][k][0], ql[R - 1][k][0], ql[0][k][1], ql[R - 1][k][1], b0, b1);
+            } else mma16816(c[0], c[1], c[2], c[3], qh[0][k][0], ql[0][k][0], qh[0][k][1], ql[0][k][1], b0, b1);
+        };
         // scores -> weights of one block: masked, scaled, running maximum; p (FP16 operand) and l
-        auto soften = [&](float (&s)[8][2 * R], uint32_t t_base, uint32_t t_end, float kscale, float vscale, bool edge, uint32_t (&p)[R][8]) {
-            const float mul = kscale * sm, lv = log2f(vscale), rv = 1.0f / vscale;
+        auto soften = [&](float (&s)[8][4], uint32_t t_base, uint32_t t_end, float mul, float lv, float rv, bool edge, uint32_t (&p)[R][8]) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float mx = -INFINITY;
@@ -362,213 +556,139 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float v = s[i][2 * r + e] * mul;
+                        if (!WIDE) s[i][e] += s[i][2 + e];
                         if (edge) {
                             const uint32_t t = t_base + 16u * j + 2u * i + e;
                             const bool vis = t < t_end && (a.window == 0u || t + a.window > (uint32_t)pos || t < a.sinks);
-                            v = vis ? v : -INFINITY;
+                            if (!vis) s[i][2 * r + e] = -INFINITY;
                         }
-                        v += lv;
-                        s[i][2 * r + e] = v;
-                        mx = fmaxf(mx, v);
+                        mx = fmaxf(mx, s[i][2 * r + e]);
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[r], mx), base = mn == -INFINITY ? 0.f : mn, back = exp2f(m[r] - base);
-                m[r] = mn;
+                mx = fmaf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), mul, lv);
+                const float mn = fmaxf(m[r], mx), shift = mn == -INFINITY ? 0.f : lv - mn;
+                if (__any_sync(0xffffffffu, mn != m[r])) {                        // a new maximum: what is summed so far shrinks
+                    const float back = mn == -INFINITY ? 1.f : fast_exp2(m[r] - mn);
+                    m[r] = mn;
+                    l[r] *= back;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) { acc[t][2 * r] *= back; acc[t][2 * r + 1] *= back; }
+                }
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float p0 = exp2f(s[i][2 * r] - base), p1 = exp2f(s[i][2 * r + 1] - base);
+                    const float p0 = fast_exp2(fmaf(s[i][2 * r], mul, shift)), p1 = fast_exp2(fmaf(s[i][2 * r + 1], mul, shift));
                     sum += p0 + p1;
                     p[r][i] = pack2(p0, p1);
                 }
-                l[r] = fmaf(l[r], back, sum * rv);
-#pragma unroll
-                for (int t = 0; t < DT; ++t) { acc[t][2 * r] *= back; acc[t][2 * r + 1] *= back; }
+                l[r] = fmaf(sum, rv, l[r]);
             }
         };
+        auto weigh = [&](int t, uint32_t (&p)[R][8], int k, uint32_t b0, uint32_t b1) {
+            float c2 = WIDE ? acc[t][2 * R - 2] : 0.f, c3 = WIDE ? acc[t][2 * R - 1] : 0.f;
+            mma16816(acc[t][0], acc[t][1], c2, c3, p[0][2 * k], WIDE ? p[R - 1][2 * k] : 0u, p[0][2 * k + 1], WIDE ? p[R - 1][2 * k + 1] : 0u, b0, b1);
+            if (WIDE) { acc[t][2 * R - 2] = c2; acc[t][2 * R - 1] = c3; }
+        };
 
-        for (uint32_t i0 = 0; i0 < n_units && ok; ++i0) {
-            const uint32_t at = at0 + i0;
-            if (at + 1u < sn.units) {
-                // ---- an 8-bit block ----
-                const uint32_t b = at < sn.sink_blocks ? at : sn.from + (at - sn.sink_blocks);
-                const float2 sc = __ldg(a.cache.scales + ch * a.cache.blocks + b);
-                const uint32_t st = consumed % kStages, ph = (consumed / kStages) & 1u, src = ring + st * BLK;
-                if (!ptx::mbar_try_wait(bar0 + 8u * st, ph)) {
-                    const long long t0 = clock64();
-                    while (ok && !ptx::mbar_try_wait(bar0 + 8u * st, ph)) ok = (unsigned long long)(clock64() - t0) < a.wait_cycles;
-                }
-                ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
-                if (!ok) break;
-                float s[8][2 * R];
-                const uint32_t tok_row = 16u * (g >> 1) + (g & 1u);
+        const uint32_t n8 = has_open ? n_units - 1u : n_units;
+        for (uint32_t i0 = 0; i0 < n8; ++i0) {
+            // ---- an 8-bit block ----
+            if (i0 && (i0 & 31u) == 0u) fetch_scales(unit0 + i0);
+            const float mul = __shfl_sync(0xffffffffu, sc_mul, i0 & 31u), lv = __shfl_sync(0xffffffffu, sc_log, i0 & 31u), rv = __shfl_sync(0xffffffffu, sc_inv, i0 & 31u);
+            const uint32_t t_base = block_of(sn, unit0 + i0) * kKv8Block;
+            const bool edge = a.window != 0u && !(t_base + a.window > (uint32_t)pos || t_base + kKv8Block <= a.sinks);
+            if (!(ok = arrived(0))) break;
+            float s[8][4];
+            const uint8_t *const k_row = granule(0) + (16u * (g >> 1) + (g & 1u)) * 64u + j * 16u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
+            for (int i = 0; i < 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
-                    for (int f = 0; f < HF; ++f) {
-                        const uint4 kk = lds16(src + f * 4096u + (tok_row + 2u * i) * 64u + j * 16u);
+            for (int f = 0; f < HF; ++f) {
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            const uint32_t w = word(kk, t), b0 = from_codes(w), b1 = from_codes(w >> 16);
-                            mma16816(c0, c1, c2, c3, qh[0][4 * f + t][0], WIDE ? qh[R - 1][4 * f + t][0] : 0u, qh[0][4 * f + t][1], WIDE ? qh[R - 1][4 * f + t][1] : 0u, b0, b1);
-                            mma16816(c0, c1, c2, c3, ql[0][4 * f + t][0], WIDE ? ql[R - 1][4 * f + t][0] : 0u, ql[0][4 * f + t][1], WIDE ? ql[R - 1][4 * f + t][1] : 0u, b0, b1);
+                for (int h = 0; h < 2; ++h) {
+                    uint4 kk[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kk[i] = *reinterpret_cast<const uint4 *>(k_row + f * 4096u + (4 * h + i) * 128u);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {                            // the tiles' chains are independent of one another
+                            const uint32_t w = word(kk[i], t);
+                            score(s[4 * h + i], 4 * f + t, from_codes(w), from_codes(w >> 16));
                         }
-                    }
-                    s[i][0] = c0; s[i][1] = c1;
-                    if (WIDE) { s[i][2 * R - 2] = c2; s[i][2 * R - 1] = c3; }
-                }
-                const uint32_t t_base = b * kKv8Block;
-                const bool edge = a.window != 0u && !(t_base + a.window > (uint32_t)pos || t_base + kKv8Block <= a.sinks);
-                uint32_t p[R][8];
-                soften(s, t_base, t_base + kKv8Block, sc.x, sc.y, edge, p);
-                uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);                     // a hidden token's codes become 0: its NaN must not count
-                if (edge) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        w[i] = 0u;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t t = t_base + 16u * j + 4u * i + e;
-                            if (t + a.window > (uint32_t)pos || t < a.sinks) w[i] |= 0xffu << (8 * e);
-                        }
-                    }
-                    keep = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    uint4 vv = lds16(src + kKv8Block * D + (8u * t + g) * 64u + j * 16u);
-                    vv.x &= keep.x; vv.y &= keep.y; vv.z &= keep.z; vv.w &= keep.w;
-                    float c2 = WIDE ? acc[t][2 * R - 2] : 0.f, c3 = WIDE ? acc[t][2 * R - 1] : 0.f;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t w = word(vv, k);
-                        mma16816(acc[t][0], acc[t][1], c2, c3, p[0][2 * k], WIDE ? p[R - 1][2 * k] : 0u, p[0][2 * k + 1], WIDE ? p[R - 1][2 * k + 1] : 0u, from_codes(w), from_codes(w >> 16));
-                    }
-                    if (WIDE) { acc[t][2 * R - 2] = c2; acc[t][2 * R - 1] = c3; }
-                }
-                __syncwarp();
-                ++consumed;
-                if (lane == 0u) issue_next();
-            } else {
-                // ---- the open block: append the new token, then attend to its FP16 rows ----
-                const uint32_t b = sn.open, slot = (uint32_t)pos % kKv8Block;
-                __half *kt = a.cache.k_tail + ch * (kKv8Block * D), *vt = a.cache.v_tail + ch * (kKv8Block * D);
-                uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + b) * BLK;
-                const bool other = a.cache.tail_block[ch] != (int)b;
-                __syncwarp();
-                if (other) {
-                    if (slot != 0u) {                                            // back inside a block already in 8 bits: its rows start from those
-                        const float2 sc = a.cache.scales[ch * a.cache.blocks + b];
-                        for (uint32_t e = lane; e < 64u * D / 2u; e += 32u) {
-                            const uint32_t k2 = e * 2u, t = (k2 >> 6) & 63u, d = (k2 >> 12) * 64u + (k2 & 63u);
-                            const float2 x = half2_of(from_codes(*reinterpret_cast<const uint16_t *>(codes + k2)));
-                            if (t < slot) *reinterpret_cast<uint32_t *>(kt + t * D + d) = pack2(x.x * sc.x, x.y * sc.x);
-                            const float2 y = half2_of(from_codes(*reinterpret_cast<const uint16_t *>(codes + kKv8Block * D + k2)));
-                            *reinterpret_cast<uint32_t *>(vt + k2) = pack2(y.x * sc.y, y.y * sc.y);
-                        }
-                    }
-                    if (lane == 0u) a.cache.tail_block[ch] = (int)b;
-                    __syncwarp();
-                }
-#pragma unroll
-                for (uint32_t p0 = 0; p0 < D / 2; p0 += 32u) {
-                    const uint32_t p = p0 + lane;
-                    float x = __half2float(a.k[((uint64_t)head * D + p) * a.pitch + col]), y = __half2float(a.k[((uint64_t)head * D + p + D / 2) * a.pitch + col]);
-                    rotate(x, y, __ldg(cs + p));
-                    kt[slot * D + p] = __float2half_rn(x);
-                    kt[slot * D + p + D / 2] = __float2half_rn(y);
-                    vt[p * 64u + slot] = a.v[((uint64_t)head * D + p) * a.pitch + col];
-                    vt[(p + D / 2) * 64u + slot] = a.v[((uint64_t)head * D + p + D / 2) * a.pitch + col];
-                }
-                __syncwarp();
-                float s[8][2 * R];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float c0 = 0.f, c1 = 0.f, c2 = 0.f, c3 = 0.f;
-                    const uint32_t tok = 16u * (g >> 1) + (g & 1u) + 2u * i;
-#pragma unroll
-                    for (int f = 0; f < HF; ++f) {
-                        uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0;
-                        if (tok <= slot) {
-                            const uint4 *row = reinterpret_cast<const uint4 *>(kt + tok * D + 64u * f + 16u * j);
-                            k0 = row[0]; k1 = row[1];
-                        }
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            const uint4 &kk = t < 2 ? k0 : k1;
-                            const uint32_t b0 = word(kk, 2 * (t & 1)), b1 = word(kk, 2 * (t & 1) + 1);
-                            mma16816(c0, c1, c2, c3, qh[0][4 * f + t][0], WIDE ? qh[R - 1][4 * f + t][0] : 0u, qh[0][4 * f + t][1], WIDE ? qh[R - 1][4 * f + t][1] : 0u, b0, b1);
-                            mma16816(c0, c1, c2, c3, ql[0][4 * f + t][0], WIDE ? ql[R - 1][4 * f + t][0] : 0u, ql[0][4 * f + t][1], WIDE ? ql[R - 1][4 * f + t][1] : 0u, b0, b1);
-                        }
-                    }
-                    s[i][0] = c0; s[i][1] = c1;
-                    if (WIDE) { s[i][2 * R - 2] = c2; s[i][2 * R - 1] = c3; }
-                }
-                uint32_t p[R][8];
-                soften(s, b * kKv8Block, (uint32_t)pos + 1u, 1.0f, 1.0f, true, p);
-                uint32_t keep[8];                                                // pairs of tokens: rows behind the last token and hidden ones become 0
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    keep[i] = 0u;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t t = b * kKv8Block + 16u * j + 2u * i + e;
-                        if (t <= (uint32_t)pos && (a.window == 0u || t + a.window > (uint32_t)pos || t < a.sinks)) keep[i] |= 0xffffu << (16 * e);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-                    if (16u * j <= slot) {
-                        const uint4 *row = reinterpret_cast<const uint4 *>(vt + (8u * t + g) * 64u + 16u * j);
-                        v0 = row[0]; v1 = row[1];
-                    }
-                    float c2 = WIDE ? acc[t][2 * R - 2] : 0.f, c3 = WIDE ? acc[t][2 * R - 1] : 0.f;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint4 &vv = k < 2 ? v0 : v1;
-                        const uint32_t b0 = word(vv, 2 * (k & 1)) & keep[2 * k], b1 = word(vv, 2 * (k & 1) + 1) & keep[2 * k + 1];
-                        mma16816(acc[t][0], acc[t][1], c2, c3, p[0][2 * k], WIDE ? p[R - 1][2 * k] : 0u, p[0][2 * k + 1], WIDE ? p[R - 1][2 * k + 1] : 0u, b0, b1);
-                    }
-                    if (WIDE) { acc[t][2 * R - 2] = c2; acc[t][2 * R - 1] = c3; }
-                }
-                if (slot == kKv8Block - 1u) {                                    // the block is whole: bring it to 8 bits
-                    float kmax = 0.f, vmax = 0.f;
-                    for (uint32_t e = lane; e < 64u * D / 8u; e += 32u) {
-                        const uint4 x = reinterpret_cast<const uint4 *>(kt)[e], y = reinterpret_cast<const uint4 *>(vt)[e];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 xf = half2_of(word(x, i)), yf = half2_of(word(y, i));
-                            kmax = amax_of(amax_of(kmax, xf.x), xf.y);
-                            vmax = amax_of(amax_of(vmax, yf.x), yf.y);
-                        }
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-                        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-                    }
-                    const float ksc = scale_of(kmax), vsc = scale_of(vmax), ki = 1.0f / ksc, vi = 1.0f / vsc;
-                    for (uint32_t e = lane; e < 64u * D / 8u; e += 32u) {
-                        const uint4 x = reinterpret_cast<const uint4 *>(kt)[e], y = reinterpret_cast<const uint4 *>(vt)[e];
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float2 x0 = half2_of(word(x, 2 * i)), x1 = half2_of(word(x, 2 * i + 1)), y0 = half2_of(word(y, 2 * i)), y1 = half2_of(word(y, 2 * i + 1));
-                            w[i] = codes4(x0.x, x0.y, x1.x, x1.y, ki);
-                            w[2 + i] = codes4(y0.x, y0.y, y1.x, y1.y, vi);
-                        }
-                        const uint32_t t = e * 8u / D, d = e * 8u % D;
-                        *reinterpret_cast<uint2 *>(codes + (d >> 6) * 4096u + t * 64u + (d & 63u)) = make_uint2(w[0], w[1]);
-                        *reinterpret_cast<uint2 *>(codes + kKv8Block * D + e * 8u) = make_uint2(w[2], w[3]);
-                    }
-                    if (lane == 0u) a.cache.scales[ch * a.cache.blocks + b] = make_float2(ksc, vsc);
                 }
             }
+            uint32_t p[R][8];
+            soften(s, t_base, t_base + kKv8Block, mul, lv, rv, edge, p);
+            release(1);
+            uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);                         // a hidden token's codes become 0: its NaN must not count
+            if (edge) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = 0u;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t t = t_base + 16u * j + 4u * i + e;
+                        if (t + a.window > (uint32_t)pos || t < a.sinks) w[i] |= 0xffu << (8 * e);
+                    }
+                }
+                keep = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (!(ok = arrived(0))) break;
+            const uint8_t *const v_row = granule(0) + g * 64u + j * 16u;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                uint4 vv = *reinterpret_cast<const uint4 *>(v_row + t * 512u);
+                vv.x &= keep.x; vv.y &= keep.y; vv.z &= keep.z; vv.w &= keep.w;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const uint32_t w = word(vv, k); weigh(t, p, k, from_codes(w), from_codes(w >> 16)); }
+            }
+            release(1);
+        }
+        if (ok && has_open) {
+            // ---- the open block: FP16 rows ----
+            const uint32_t b = sn.open;
+            if (lane == 0u) a.cache.tail_block[ch] = (int)b;
+            ok = arrived(0) && arrived(1);
+            if (!ok) break;
+            const __half *g0 = reinterpret_cast<const __half *>(granule(0)), *g1 = reinterpret_cast<const __half *>(granule(1));       // keys: tokens 0 .. 31, 32 .. 63
+            float s[8][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+            const __half *k_row = (g < 4u ? g0 : g1) + (16u * ((g >> 1) & 1u) + (g & 1u)) * D + 16u * j;      // token 16 (g / 2) + g % 2 + 2 i
+#pragma unroll
+            for (int f = 0; f < HF; ++f)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 k0 = *reinterpret_cast<const uint4 *>(k_row + 64 * f + 2 * i * D), k1 = *reinterpret_cast<const uint4 *>(k_row + 64 * f + 2 * i * D + 8);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) { const uint4 &kk = t < 2 ? k0 : k1; score(s[i], 4 * f + t, word(kk, 2 * (t & 1)), word(kk, 2 * (t & 1) + 1)); }
+                }
+            uint32_t p[R][8];
+            soften(s, b * kKv8Block, (uint32_t)pos + 1u, sm, 0.f, 1.0f, true, p);
+            release(2);
+            ok = arrived(0) && arrived(1);
+            if (!ok) break;
+            g0 = reinterpret_cast<const __half *>(granule(0)); g1 = reinterpret_cast<const __half *>(granule(1));      // values: the first and the second half of the dimensions
+            uint32_t keep[8];                                                    // pairs of tokens: rows behind the last token and hidden ones become 0
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                keep[i] = 0u;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t t = b * kKv8Block + 16u * j + 2u * i + e;
+                    if (t <= (uint32_t)pos && (a.window == 0u || t + a.window > (uint32_t)pos || t < a.sinks)) keep[i] |= 0xffffu << (16 * e);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const uint4 *row = reinterpret_cast<const uint4 *>((t < DT / 2 ? g0 : g1) + (8u * (t % (DT / 2)) + g) * 64u + 16u * j);
+                const uint4 v0 = row[0], v1 = row[1];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { const uint4 &vv = k < 2 ? v0 : v1; weigh(t, p, k, word(vv, 2 * (k & 1)) & keep[2 * k], word(vv, 2 * (k & 1) + 1) & keep[2 * k + 1]); }
+            }
+            release(2);
         }
         if (!ok) break;
         // ---- this part is done: the output, or a part of it ----
@@ -577,63 +697,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
         }
-        bool write = n_units == sn.units;
-        if (!write) {
-            // slot 0 belongs to the (column, head) that holds this warp's first unit, slot 1 to the other one it may share
-            float *mine = a.partial + ((uint64_t)me * 2u + (u == u_begin ? 0u : 1u)) * (GP * PROW);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float *row = mine + (g + 8u * r) * PROW;
-                if (g + 8u * r < G) {
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) __stcg(reinterpret_cast<float2 *>(row + 8u * t + 2u * j), make_float2(acc[t][2 * r], acc[t][2 * r + 1]));
-                    if (j == 0u) __stcg(reinterpret_cast<float2 *>(row + D), make_float2(m[r], l[r]));
-                }
-            }
-            __threadfence();
-            __syncwarp();
-            uint32_t before = 0;
-            if (lane == 0u) before = atomicAdd(a.counters + ch, n_units);
-            before = __shfl_sync(0xffffffffu, before, 0);
-            if (before + n_units == sn.units) {                                  // all parts are there
-                __threadfence();
-                if (lane == 0u) a.counters[ch] = 0u;
-                const uint32_t w0 = worker_of(seg0), w1 = worker_of(seg0 + sn.units - 1u);
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    m[r] = -INFINITY; l[r] = 0.f;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) { acc[t][2 * r] = 0.f; acc[t][2 * r + 1] = 0.f; }
-                }
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const uint32_t row = g + 8u * r;
-                    for (uint32_t w = w0 + j; w <= w1 && row < G; w += 4u) {
-                        const float *src = a.partial + ((uint64_t)w * 2u + (share(w) >= seg0 ? 0u : 1u)) * (GP * PROW) + row * PROW;
-                        m[r] = fmaxf(m[r], __ldcg(src + D));
-                    }
-                    m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
-                    m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2));
-                    const float base = m[r] == -INFINITY ? 0.f : m[r];
-                    if (row < G) {
-                        for (uint32_t w = w0; w <= w1; ++w) {
-                            const float *src = a.partial + ((uint64_t)w * 2u + (share(w) >= seg0 ? 0u : 1u)) * (GP * PROW) + row * PROW;
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(src + D));
-                            const float f = exp2f(ml.x - base);
-                            l[r] = fmaf(ml.y, f, l[r]);
-#pragma unroll
-                            for (int t = 0; t < DT; ++t) {
-                                const float2 x = __ldcg(reinterpret_cast<const float2 *>(src + 8u * t + 2u * j));
-                                acc[t][2 * r] = fmaf(x.x, f, acc[t][2 * r]);
-                                acc[t][2 * r + 1] = fmaf(x.y, f, acc[t][2 * r + 1]);
-                            }
-                        }
-                    }
-                }
-                write = true;
-            }
-        }
-        if (write) {
+        if (n_units == sn.units) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const uint32_t row = g + 8u * r;
@@ -647,8 +711,68 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
                     }
                 }
             }
+        } else {
+            // slot 0 belongs to the (column, head) in which this warp's share begins, slot 1 to the other one it may split with a neighbour
+            float *own = a.partial + ((uint64_t)me * 2u + (x_begin >= seg0 ? 0u : 1u)) * (GP * PROW);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const uint32_t row = g + 8u * r;
+                if (row < G) {
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) __stcg(reinterpret_cast<float2 *>(own + row * D + 8u * t + 2u * j), make_float2(acc[t][2 * r], acc[t][2 * r + 1]));
+                    if (j == 0u) __stcg(reinterpret_cast<float2 *>(own + GP * D + 2u * row), make_float2(m[r], l[r]));
+                }
+            }
+            __threadfence();
+            __syncwarp();
+            uint32_t before = 0;
+            if (lane == 0u) before = atomicAdd(a.counters + ch, n_units);
+            before = __shfl_sync(0xffffffffu, before, 0);
+            if (before + n_units == sn.units) {                                  // all parts are there
+                __threadfence();
+                if (lane == 0u) a.counters[ch] = 0u;
+                const uint32_t w0 = worker_of(seg0), n = worker_of(seg0 + sn.units - 1u) - w0 + 1u;
+                auto part = [&](uint32_t i) -> const float * { return a.partial + ((uint64_t)(w0 + i) * 2u + (share(w0 + i) >= seg0 ? 0u : 1u)) * (GP * PROW); };
+                // a lane takes four dimensions of a row, the parts in their order, four of them in flight (short code: it is fetched cold)
+                for (uint32_t e = lane * 4u; e < G * D; e += 128u) {
+                    const uint32_t row = e / D;
+                    float M = -INFINITY, L = 0.f;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                    for (uint32_t i0 = 0; i0 < n; i0 += 4u) {
+                        float2 ml[4];
+                        float4 x[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i) {
+                            ml[i] = make_float2(-INFINITY, 0.f);
+                            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (i0 + i < n) {
+                                const float *src = part(i0 + i);
+                                ml[i] = __ldcg(reinterpret_cast<const float2 *>(src + GP * D + 2u * row));
+                                x[i] = __ldcg(reinterpret_cast<const float4 *>(src + e));
+                            }
+                        }
+                        const float mn = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), to = mn == -INFINITY ? 0.f : mn, back = fast_exp2(M - to);
+                        M = mn;
+                        L *= back; o.x *= back; o.y *= back; o.z *= back; o.w *= back;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i) {
+                            const float f = fast_exp2(ml[i].x - to);
+                            L = fmaf(ml[i].y, f, L);
+                            o.x = fmaf(x[i].x, f, o.x); o.y = fmaf(x[i].y, f, o.y); o.z = fmaf(x[i].z, f, o.z); o.w = fmaf(x[i].w, f, o.w);
+                        }
+                    }
+                    const float inv = 1.0f / L;
+                    __half *dst = a.out + ((uint64_t)head * G * D + e) * a.pitch + col;
+                    dst[0] = __float2half_rn(o.x * inv);
+                    dst[a.pitch] = __float2half_rn(o.y * inv);
+                    dst[2ull * a.pitch] = __float2half_rn(o.z * inv);
+                    dst[3ull * a.pitch] = __float2half_rn(o.w * inv);
+                }
+            }
         }
-        u += n_units;
+        if (has_open) next_head(at);
+        else { at.unit += n_units; at.x += n_units; }
     }
     if (!ok) {                                                                    // gave up: report, wait (bounded) for own copies, leave
         if (lane == 0u) {
@@ -656,7 +780,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
             for (uint32_t i = consumed; i < issued; ++i) {
                 const long long t0 = clock64();
                 bool done = false;
-                while (!done && (unsigned long long)(clock64() - t0) < a.wait_cycles) done = ptx::mbar_try_wait(bar0 + 8u * (i % kStages), (i / kStages) & 1u);
+                while (!done && (unsigned long long)(clock64() - t0) < a.wait_cycles) done = ptx::mbar_try_wait(bar0 + 8u * (i % RING), (i / RING) & 1u);
                 if (!done) atomicOr(a.status, (uint32_t)ST_TIMEOUT_DRAIN);
             }
         }
@@ -664,8 +788,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) k44_kv8_attn_kernel(const Kv8At
     }
 }
 
-template <int D, int WARPS>
-constexpr uint32_t attn_smem(uint32_t columns) { return WARPS * kStages * 2u * kKv8Block * D + (columns + 1u) * 4u; }
+template <int D, bool WIDE> constexpr uint32_t attn_smem(uint32_t columns) { return kWarps<D, WIDE> * kRing<D, WIDE> * kKv8Block * D + (columns + 1u) * 4u; }
+template <int D, bool WIDE> constexpr uint32_t kPrepareSmem = 8u * (8u * (WIDE ? 2u : 1u) * D + 8u) * 2u;
+template <int D, bool WIDE> cudaError_t attn_setup() {
+    return cudaFuncSetAttribute(k44_kv8_attn_kernel<D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem<D, WIDE>(kKv8MaxColumns));
+}
+template <int D, bool WIDE> cudaError_t attn_launch(const Kv8AttnArgs &a, uint32_t num_sms, bool pdl, cudaStream_t s) {
+    Kv8AttnArgs b = a;
+    b.workers = num_sms * kWarps<D, WIDE>;
+    b.spread = (uint32_t)(0.6180339887 * b.workers);
+    while (std::gcd(b.spread, b.workers) != 1u) ++b.spread;
+    const cudaError_t e = launch_dep(k44_kv8_prepare_kernel<D, WIDE>, dim3((a.columns + 7u) / 8u, a.cache.h_kv, 3), dim3(256), kPrepareSmem<D, WIDE>, pdl, s, b);
+    if (e != cudaSuccess) return e;
+    return launch_dep(k44_kv8_attn_kernel<D, WIDE>, dim3(num_sms), dim3(kWarps<D, WIDE> * 32u), attn_smem<D, WIDE>(a.columns), pdl, s, b);
+}
 
 }  // namespace
 
@@ -682,25 +818,25 @@ cudaError_t launch_kv8_fill(const Kv8FillArgs &a, bool pdl, cudaStream_t s) {
 }
 
 cudaError_t kv8_attn_setup() {
-    cudaError_t e = cudaFuncSetAttribute(k44_kv8_attn_kernel<64, kWarps64, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem<64, kWarps64>(kKv8MaxColumns));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k44_kv8_attn_kernel<64, kWarps64, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem<64, kWarps64>(kKv8MaxColumns));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k44_kv8_attn_kernel<128, kWarps128, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem<128, kWarps128>(kKv8MaxColumns));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k44_kv8_attn_kernel<128, kWarps128, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem<128, kWarps128>(kKv8MaxColumns));
-    return e;
+    for (cudaError_t e : {attn_setup<64, false>(), attn_setup<64, true>(), attn_setup<128, false>(), attn_setup<128, true>()})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
+}
+
+uint64_t kv8_attn_frag_bytes(uint32_t columns, uint32_t h_kv, uint32_t group, uint32_t head_dim) {
+    return (uint64_t)columns * h_kv * (group > 8u ? 2u : 1u) * (head_dim / 16u) * 32u * sizeof(uint4);
 }
 
 uint64_t kv8_attn_partial_bytes(uint32_t num_sms, uint32_t group, uint32_t head_dim) {
-    return (uint64_t)num_sms * (head_dim == 64u ? kWarps64 : kWarps128) * 2u * (group > 8u ? 16u : 8u) * (head_dim + 2u) * sizeof(float);
+    const bool wide = group > 8u;
+    const uint32_t warps = head_dim == 64u ? (wide ? kWarps<64, true> : kWarps<64, false>) : (wide ? kWarps<128, true> : kWarps<128, false>);
+    return (uint64_t)num_sms * warps * 2u * (wide ? 16u : 8u) * (head_dim + 2u) * sizeof(float);
 }
 
 cudaError_t launch_kv8_attn(const Kv8AttnArgs &a, uint32_t num_sms, bool pdl, cudaStream_t s) {
     const bool wide = a.h_q / a.cache.h_kv > 8u;
-    const dim3 grid(num_sms);
-    if (a.cache.head_dim == 64u)
-        return wide ? launch_dep(k44_kv8_attn_kernel<64, kWarps64, true>, grid, dim3(kWarps64 * 32u), attn_smem<64, kWarps64>(a.columns), pdl, s, a)
-                    : launch_dep(k44_kv8_attn_kernel<64, kWarps64, false>, grid, dim3(kWarps64 * 32u), attn_smem<64, kWarps64>(a.columns), pdl, s, a);
-    return wide ? launch_dep(k44_kv8_attn_kernel<128, kWarps128, true>, grid, dim3(kWarps128 * 32u), attn_smem<128, kWarps128>(a.columns), pdl, s, a)
-                : launch_dep(k44_kv8_attn_kernel<128, kWarps128, false>, grid, dim3(kWarps128 * 32u), attn_smem<128, kWarps128>(a.columns), pdl, s, a);
+    if (a.cache.head_dim == 64u) return wide ? attn_launch<64, true>(a, num_sms, pdl, s) : attn_launch<64, false>(a, num_sms, pdl, s);
+    return wide ? attn_launch<128, true>(a, num_sms, pdl, s) : attn_launch<128, false>(a, num_sms, pdl, s);
 }
 
 }  // namespace k44b
