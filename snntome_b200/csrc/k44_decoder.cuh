@@ -101,13 +101,16 @@ struct LogprobArgs {
     int *top_rows = nullptr;
     float4 *parts = nullptr;                         // [column][chunk]: maximum, sum of e^(x - max), sum of e^(x - max) (x - max)
     uint16_t *group_max = nullptr;                   // [column][group]: order of the largest value of 64 rows
-    uint32_t rows = 0, pitch = 0, columns = 0, top = 0, chunks = 0, groups = 0;
+    uint32_t *status = nullptr;
+    unsigned long long wait_cycles = 0;
+    uint32_t rows = 0, pitch = 0, columns = 0, top = 0, chunks = 0, groups = 0, chunk_groups = 0, group_stride = 0;
 };
-constexpr uint32_t kLogprobGroup = 64, kLogprobChunk = 512, kLogprobTop = 32;
-constexpr uint32_t kLogprobMaxRows = 65535u * kLogprobGroup;
-uint64_t logprob_scratch_bytes(uint32_t rows, uint32_t columns);
-void logprob_place(LogprobArgs &a, void *scratch);
-cudaError_t launch_logprobs(const LogprobArgs &a, bool pdl, cudaStream_t s);
+constexpr uint32_t kLogprobGroup = 64, kLogprobTop = 32;
+constexpr uint32_t kLogprobMaxRows = 65528u * kLogprobGroup;           // a group's number in 16 bits
+uint64_t logprob_scratch_bytes(uint32_t rows, uint32_t columns, uint32_t num_sms);
+void logprob_place(LogprobArgs &a, void *scratch, uint32_t num_sms);
+cudaError_t logprob_setup();
+cudaError_t launch_logprobs(const LogprobArgs &a, const CUtensorMap &map, bool pdl, cudaStream_t s);      // map: the logits as rows of `pitch`, boxes of 64 x 64
 
 // programmatic dependent launch, as in k44_valu.cu
 __device__ __forceinline__ void dep_enter() {

@@ -683,11 +683,13 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         for (const auto &p : arrays) if (p.first && !device_memory(p.first, p.second)) return bad(err);
         reads(w.src_off, w.cout);
         LogprobArgs &a = dw.logprob;
+        a.status = d_status_; a.wait_cycles = wait_cycles;
+        if (!check(logprob_setup(), "kernel attribute setup") || !encode_map_2d(&dw.logit_map, canvas_ + w.src_off, pitch_, w.cout, 64u, 64u, false)) return false;
         a.x = canvas_ + w.src_off; a.rows = w.cout; a.pitch = pitch_; a.columns = columns_; a.top = w.top;
         a.targets = w.targets; a.logprobs = w.logprobs; a.entropy = w.entropy; a.top_rows = w.top_rows; a.top_logprobs = w.top_logprobs;
-        if (!reserve(d_logprob_, logprob_bytes_, logprob_scratch_bytes(w.cout, columns_), "probability scratch allocation")) return false;
-        logprob_place(a, d_logprob_);
-        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_LOGPROBS) logprob_place(o.logprob, d_logprob_);
+        if (!reserve(d_logprob_, logprob_bytes_, logprob_scratch_bytes(w.cout, columns_, (uint32_t)num_sms_), "probability scratch allocation")) return false;
+        logprob_place(a, d_logprob_, (uint32_t)num_sms_);
+        for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_LOGPROBS) logprob_place(o.logprob, d_logprob_, (uint32_t)num_sms_);
         return true;
     }
     default: return fail("unknown command kind");
@@ -1208,7 +1210,7 @@ bool Executor::launch_one(DeviceWave &w, cudaStream_t stream, uint32_t peer_slac
         case AUX_WINDOW_ATTN: launches_ += 2u; return check(launch_window_attn(w.window, w.window_maps, pdl_, stream), what.c_str());
         case AUX_KV8_FILL: ++launches_; return check(launch_kv8_fill(w.fill, pdl_, stream), what.c_str());
         case AUX_KV8_ATTN: launches_ += 2u; return check(launch_kv8_attn(w.kv8, (uint32_t)num_sms_, pdl_, stream), what.c_str());
-        case AUX_LOGPROBS: launches_ += 2u; return check(launch_logprobs(w.logprob, pdl_, stream), what.c_str());
+        case AUX_LOGPROBS: launches_ += 2u; return check(launch_logprobs(w.logprob, w.logit_map, pdl_, stream), what.c_str());
         default: break;
         }
         launches_ += (w.aux.kind == AUX_ROPE_ATTN || w.aux.kind == AUX_DECODE_ATTN) ? 3u : (w.aux.kind == AUX_ARGMAX ? 2u : 1u);

@@ -47,6 +47,7 @@ struct DeviceWave {
     Kv8FillArgs fill;                    // 14: prompt keys / values into an 8-bit cache
     Kv8AttnArgs kv8;                     // 15: single tokens against it
     LogprobArgs logprob;                 // 16: answer probabilities
+    CUtensorMap logit_map;
     WaveArgs args;
     UmmaDesc desc;
     CUtensorMap tmap;
