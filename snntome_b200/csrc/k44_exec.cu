@@ -593,7 +593,7 @@ bool Executor::place_window(DeviceWave &dw) {
     auto rows = [&](CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint32_t box_rows) {
         return encode_map_2d(map, base, inner, outer, 64u, box_rows);
     };
-    return rows(&dw.window_maps.q, a.q_rows, a.head_dim, (uint64_t)a.h_q * a.pitch, 128u) && rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 128u) &&
+    return rows(&dw.window_maps.q, a.q_rows, a.head_dim, (uint64_t)a.h_q * a.pitch, 128u) && rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 64u) &&
            rows(&dw.window_maps.v, a.v_rows, a.pitch, (uint64_t)a.h_kv * a.head_dim, a.head_dim);
 }
 

@@ -6,7 +6,7 @@
 //
 // Two launches. The first rotates q and k and lays them out token by token (the rows a tensor-core operand wants), and copies v;
 // q, k and v on the canvas stay as they are. The second is the attention: a CTA owns 128 columns of one query head and walks
-// the tiles of 128 keys that any of its columns sees — hidden tiles are never read. Tiles are cut at multiples of 128 canvas
+// the tiles of 64 keys that any of its columns sees — hidden tiles are never read. Tiles are cut at multiples of 64 canvas
 // columns whatever the sequences' lengths, so that every copy is aligned; sequences that end inside a tile cost a mask.
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
@@ -19,18 +19,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) != 0x7c00u; }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
-// CTA = 64 columns of one head of q, k or v. Columns behind the plan's last one become zero. Values that are not finite become
+// CTA = 64 columns of a few heads of q and k, or of one head of v. Columns behind the plan's last one become zero. Values that are not finite become
 // zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the tensor cores;
 // the attention adds them to the columns that do see them.
 template <int D>
-__global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a) {
+__global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a, uint32_t heads) {
     dep_enter();
-    constexpr int ROW = 64 + 8;
+    constexpr int ROW = 64 + 2;                                     // 33 words: pairs 8 rows apart fall on different banks
     __shared__ __align__(16) __half xs[D * ROW];
-    const uint32_t tile = blockIdx.x, tid = threadIdx.x, col0 = tile * 64u;
-    uint32_t h = blockIdx.y;
-    if (h >= a.h_q + a.h_kv) {
-        h -= a.h_q + a.h_kv;
+    const uint32_t tile = blockIdx.x, tid = threadIdx.x, col0 = tile * 64u, turned = (a.h_q + a.h_kv + heads - 1u) / heads;
+    uint32_t h = blockIdx.y * heads;
+    if (blockIdx.y >= turned) {
+        h = blockIdx.y - turned;
         const __half *src = a.v + (uint64_t)h * D * a.pitch + col0;
         __half *dst = a.v_rows + (uint64_t)h * D * a.pitch + col0;
         uint32_t bad = 0;
@@ -52,48 +52,85 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
         if (tid == 0u) a.v_flags[h * (a.pitch / 64u) + tile] = any ? 1u : 0u;
         return;
     }
-    const bool is_q = h < a.h_q;
-    if (!is_q) h -= a.h_q;
-    const __half *src = (is_q ? a.q : a.k) + (uint64_t)h * D * a.pitch + col0;
-    __half *dst = (is_q ? a.q_rows : a.k_rows) + ((uint64_t)h * a.pitch + col0) * D;
-    for (uint32_t e = tid; e < D * 8u; e += 256u) {
-        const uint32_t d = e >> 3, c = (e & 7u) * 8u;
-        *reinterpret_cast<uint4 *>(xs + d * ROW + c) = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
-    }
-    __syncthreads();
-    // a thread owns one token and runs of 8 pairs: 16 bytes of either half of the row
-    const uint32_t tok = tid & 63u, col = col0 + tok;
-    const bool live = col < a.columns;
-    const float2 *cs = a.rope + (uint64_t)(col % a.seq_len) * (D / 2);
-    for (uint32_t p0 = (tid >> 6) * 8u; p0 < D / 2; p0 += 32u) {
-        __half lo[8], hi[8];
+    // A thread owns one token and 8 rotation pairs (16 bytes of either half of the token's row); neighbours own the next pairs, so that
+    // table and rows are read and written in whole lines. Its angles serve every head of the CTA.
+    constexpr uint32_t PER = D / 16, TOKENS = 256u / PER, ROUNDS = 64u / TOKENS;
+    const uint32_t part = tid % PER, p0 = part * 8u;
+    float2 cs[ROUNDS][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = __half2float(xs[(p0 + i) * ROW + tok]), y = __half2float(xs[(p0 + i + D / 2) * ROW + tok]);
-            const float2 r = live ? __ldg(cs + p0 + i) : make_float2(0.f, 0.f);
-            lo[i] = __float2half_rn(live ? x * r.x - y * r.y : 0.f);
-            hi[i] = __float2half_rn(live ? x * r.y + y * r.x : 0.f);
+    for (uint32_t n = 0; n < ROUNDS; ++n) {
+        const uint32_t col = col0 + n * TOKENS + tid / PER;
+        const float4 *from = reinterpret_cast<const float4 *>(a.rope + (uint64_t)(col % a.seq_len) * (D / 2) + p0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = col < a.columns ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            cs[n][2 * i] = make_float2(v.x, v.y);
+            cs[n][2 * i + 1] = make_float2(v.z, v.w);
         }
-        *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0) = *reinterpret_cast<uint4 *>(lo);
-        *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0 + D / 2) = *reinterpret_cast<uint4 *>(hi);
+    }
+    const uint32_t h0 = h, h1 = min(h0 + heads, a.h_q + a.h_kv);
+    uint4 next[D / 32];                                                      // the rows of the head after this one
+    auto fetch = [&](uint32_t i) {
+        const __half *src = (i < a.h_q ? a.q + (uint64_t)i * D * a.pitch : a.k + (uint64_t)(i - a.h_q) * D * a.pitch) + col0;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) { const uint32_t e = 256u * n + tid; next[n] = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)(e >> 3) * a.pitch + (e & 7u) * 8u)); }
+    };
+    fetch(h0);
+    for (h = h0; h < h1; ++h) {
+        const bool is_q = h < a.h_q;
+        const uint32_t head = is_q ? h : h - a.h_q;
+        __half *dst = (is_q ? a.q_rows : a.k_rows) + ((uint64_t)head * a.pitch + col0) * D;
+        if (h != h0) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const uint32_t e = 256u * n + tid;
+            uint32_t *to = reinterpret_cast<uint32_t *>(xs + (e >> 3) * ROW + (e & 7u) * 8u);
+            to[0] = next[n].x; to[1] = next[n].y; to[2] = next[n].z; to[3] = next[n].w;
+        }
+        __syncthreads();
+        if (h + 1u < h1) fetch(h + 1u);
+#pragma unroll
+        for (uint32_t n = 0; n < ROUNDS; ++n) {
+            const uint32_t tok = n * TOKENS + tid / PER;
+            const bool live = col0 + tok < a.columns;
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float u[2], v[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x = __half2float(xs[(p0 + 2 * i + e) * ROW + tok]), y = __half2float(xs[(p0 + 2 * i + e + D / 2) * ROW + tok]);
+                    const float2 r = cs[n][2 * i + e];
+                    u[e] = live ? x * r.x - y * r.y : 0.f;
+                    v[e] = live ? x * r.y + y * r.x : 0.f;
+                }
+                const __half2 l2 = __floats2half2_rn(u[0], u[1]), h2 = __floats2half2_rn(v[0], v[1]);
+                lo[i] = *reinterpret_cast<const uint32_t *>(&l2);
+                hi[i] = *reinterpret_cast<const uint32_t *>(&h2);
+            }
+            *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4 *>(dst + (uint64_t)tok * D + p0 + D / 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        }
     }
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------------------
 // Warp 0 copies (TMA), one thread of warp 1 issues the MMAs, warps 2-5 are the softmax: a thread owns one column (= TMEM lane).
-// Tensor memory: 128 columns of scores, over whose first half the weights are written as FP16 pairs once they are read (the A
-// operand of the second product), and D columns of output. That is half of the SM's, so two CTAs share an SM and one's
-// exponentials run under the other's products: per tile 128 x 128 exponentials take 1024 cycles of the SM's 16 per cycle, the
-// products 256 (D = 64) — the exponentials bound this kernel, not the tensor cores.
+// Tensor memory: two buffers of 64 columns of scores, over whose first half the weights are written as FP16 pairs once the scores
+// are read (the A operand of the second product), and D columns of output. That is half of the SM's, so two CTAs share an SM. While
+// the softmax works on one buffer the next scores are already being made in the other, so that its warps wait for nothing of their
+// own CTA's but their own loads, and those hide behind the other CTA's exponentials: 128 x 128 of them take 1024 cycles of the SM's 16
+// per cycle, their products 256 (D = 64) — the exponentials bound this kernel, not the tensor cores. (One buffer of 128 keys per CTA:
+// 2340 cycles.)
 // The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
 // exact in FP16 as weights up to 1, and the sum is kept against the same maximum.
 template <int D> struct Shape {
     static constexpr uint32_t HF = D / 64;
-    static constexpr uint32_t Q_BYTES = 128u * D * 2u, K_BYTES = Q_BYTES, V_BYTES = Q_BYTES;
-    static constexpr uint32_t STAGES = D == 64 ? 2u : 1u;
+    static constexpr uint32_t Q_BYTES = 128u * D * 2u, K_BYTES = 64u * D * 2u, V_BYTES = K_BYTES;
+    static constexpr uint32_t STAGES = D == 64 ? 4u : 2u;
     static constexpr uint32_t SMEM = Q_BYTES + STAGES * (K_BYTES + V_BYTES) + 1024u + 256u;
 };
-constexpr uint32_t kThreads = 192, kTmemCols = 256, kOCol = 128;
+constexpr uint32_t kThreads = 192, kTmemCols = 256, kOCol = 128, kKeys = 64;
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
     // K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
@@ -103,6 +140,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// bits from .. to of a word (either may lie outside it)
+__device__ __forceinline__ uint32_t bits(int from, int to) {
+    if (to < 0 || from > 31 || from > to) return 0u;
+    return (0xffffffffu >> (31 - min(to, 31))) & (0xffffffffu << max(from, 0));
 }
 
 template <int D>
@@ -114,9 +156,9 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     const uint32_t base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_smem = base, k_smem = q_smem + S::Q_BYTES, v_smem = k_smem + ST * S::K_BYTES, ctl = v_smem + ST * S::V_BYTES;
     const uint32_t q_full = ctl, k_full = ctl + 8u, k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST;
-    const uint32_t s_full = v_empty + 8u * ST, p_full = s_full + 8u, o_full = p_full + 8u;
+    const uint32_t s_full = v_empty + 8u * ST, p_full = s_full + 16u, pv_done = p_full + 16u;
     uint8_t *ctl_ptr = smem_raw + (ctl - ptx::smem_addr(smem_raw));
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(ctl_ptr + 128), *abort_word = tmem_slot + 1;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(ctl_ptr + 192), *abort_word = tmem_slot + 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0) {
@@ -125,7 +167,8 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             ptx::mbar_init(k_full + 8u * s, 1); ptx::mbar_init(k_empty + 8u * s, 1);
             ptx::mbar_init(v_full + 8u * s, 1); ptx::mbar_init(v_empty + 8u * s, 1);
         }
-        ptx::mbar_init(s_full, 1); ptx::mbar_init(p_full, 128); ptx::mbar_init(o_full, 1);
+        for (uint32_t b = 0; b < 2u; ++b) { ptx::mbar_init(s_full + 8u * b, 1); ptx::mbar_init(p_full + 8u * b, 128); }
+        ptx::mbar_init(pv_done, 1);
         *abort_word = 0;
         ptx::fence_mbar_init();
     }
@@ -156,10 +199,10 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     const bool one_seq = t_last - s_first < a.seq_len;
     uint32_t lo_first = s_first;
     if (a.window && t_first - s_first >= a.window) lo_first = t_first - a.window + 1u;
-    const uint32_t w_tile = lo_first / 128u;
-    uint32_t n_sink = 0, sink_tile = s_first / 128u;
-    if (a.window && a.sinks && sink_tile < w_tile) n_sink = min(w_tile, (s_first + min(a.sinks, a.seq_len) - 1u) / 128u + 1u) - sink_tile;
-    const uint32_t n = n_sink + (qt - w_tile + 1u);
+    const uint32_t w_tile = lo_first / kKeys, sink_tile = s_first / kKeys;
+    uint32_t n_sink = 0;
+    if (a.window && a.sinks && sink_tile < w_tile) n_sink = min(w_tile, (s_first + min(a.sinks, a.seq_len) - 1u) / kKeys + 1u) - sink_tile;
+    const uint32_t n = n_sink + (t_last / kKeys - w_tile + 1u);
     auto key_tile = [&](uint32_t j) -> uint32_t { return j < n_sink ? sink_tile + j : w_tile + (j - n_sink); };
 
     bool ok = true;
@@ -170,14 +213,14 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(q_smem + f * 16384u, &q_map, (int32_t)(64u * f), (int32_t)(hq * a.pitch + t_first), q_full, keep);
             uint32_t k_issued = 0, v_issued = 0;
             for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t s = j % ST, ph = (j / ST) & 1u, c0 = key_tile(j) * 128u;
+                const uint32_t s = j % ST, ph = (j / ST) & 1u, c0 = key_tile(j) * kKeys;
                 if (!(ok = wait(k_empty + 8u * s, ph ^ 1u))) break;
                 ptx::mbar_arrive_expect_tx(k_full + 8u * s, S::K_BYTES);
-                for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(k_smem + s * S::K_BYTES + f * 16384u, &k_map, (int32_t)(64u * f), (int32_t)(hk * a.pitch + c0), k_full + 8u * s, keep);
+                for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(k_smem + s * S::K_BYTES + f * 8192u, &k_map, (int32_t)(64u * f), (int32_t)(hk * a.pitch + c0), k_full + 8u * s, keep);
                 ++k_issued;
                 if (!(ok = wait(v_empty + 8u * s, ph ^ 1u))) break;
                 ptx::mbar_arrive_expect_tx(v_full + 8u * s, S::V_BYTES);
-                for (uint32_t f = 0; f < 2u; ++f) ptx::tma_load_2d(v_smem + s * S::V_BYTES + f * (D * 128u), &v_map, (int32_t)(c0 + 64u * f), (int32_t)(hk * D), v_full + 8u * s, keep);
+                ptx::tma_load_2d(v_smem + s * S::V_BYTES, &v_map, (int32_t)c0, (int32_t)(hk * D), v_full + 8u * s, keep);
                 ++v_issued;
             }
             if (!ok) {
@@ -198,24 +241,29 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
-            ok = wait(q_full, 0u);
-            for (uint32_t j = 0; j < n && ok; ++j) {
-                const uint32_t s = j % ST, ph = (j / ST) & 1u;
-                if (!(ok = wait(k_full + 8u * s, ph))) break;
+            constexpr uint32_t idesc_s = (1u << 4) | ((kKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+            auto scores = [&](uint32_t j) -> bool {
+                const uint32_t s = j % ST, to = tmem + (j & 1u) * kKeys;
+                if (!wait(k_full + 8u * s, (j / ST) & 1u)) return false;
                 ptx::tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < D / 16u; ++k)
-                    ptx::umma_f16(tmem, desc_sw128(q_smem + (k >> 2) * 16384u) + (k & 3u) * 2u, desc_sw128(k_smem + s * S::K_BYTES + (k >> 2) * 16384u) + (k & 3u) * 2u, idesc_s, k != 0u ? 1u : 0u);
+                    ptx::umma_f16(to, desc_sw128(q_smem + (k >> 2) * 16384u) + (k & 3u) * 2u, desc_sw128(k_smem + s * S::K_BYTES + (k >> 2) * 8192u) + (k & 3u) * 2u, idesc_s, k != 0u ? 1u : 0u);
                 ptx::umma_commit(k_empty + 8u * s);
-                ptx::umma_commit(s_full);
-                if (!(ok = wait(v_full + 8u * s, ph) && wait(p_full, j & 1u))) break;
+                ptx::umma_commit(s_full + 8u * (j & 1u));
+                return true;
+            };
+            ok = wait(q_full, 0u) && scores(0u) && (n < 2u || scores(1u));
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                const uint32_t s = j % ST;
+                if (!(ok = wait(v_full + 8u * s, (j / ST) & 1u) && wait(p_full + 8u * (j & 1u), (j >> 1) & 1u))) break;
                 ptx::tc_fence_after();
 #pragma unroll
-                for (uint32_t k = 0; k < 8u; ++k)
-                    ptx::umma_f16_a_tmem(tmem + kOCol, tmem + 8u * k, desc_sw128(v_smem + s * S::V_BYTES + (k >> 2) * (D * 128u)) + (k & 3u) * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
+                for (uint32_t k = 0; k < kKeys / 16u; ++k)
+                    ptx::umma_f16_a_tmem(tmem + kOCol, tmem + (j & 1u) * kKeys + 8u * k, desc_sw128(v_smem + s * S::V_BYTES) + k * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
                 ptx::umma_commit(v_empty + 8u * s);
-                if (j + 1u == n) ptx::umma_commit(o_full);
+                ptx::umma_commit(pv_done);
+                if (j + 2u < n) ok = scores(j + 2u);                        // over the weights that the product before it has read
             }
             if (!ok) {
                 if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_MMA);
@@ -229,41 +277,47 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         const float mul = rsqrtf((float)D) * kLog2e;
         // what column t sees: [lo, t] and [s0, s0 + sk)
         const uint32_t s0 = t / a.seq_len * a.seq_len;
-        const uint32_t lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0, span = t - lo + 1u;
+        const uint32_t lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0;
         const uint32_t sk = lo > s0 ? min(a.sinks, lo - s0) : 0u;
+        auto seen = [&](uint32_t c0) -> uint32_t {                          // of the 32 keys from c0
+            const int at = (int)c0;
+            return bits((int)lo - at, (int)t - at) | bits((int)s0 - at, (int)(s0 + sk) - 1 - at);
+        };
         float m = -INFINITY, l = 0.f;                                     // maximum that the weights are kept against (scaled), their sum
         for (uint32_t j = 0; j < n && ok; ++j) {
-            const uint32_t c0 = key_tile(j) * 128u;
+            const uint32_t c0 = key_tile(j) * kKeys, from = lane_base + (j & 1u) * kKeys;
             // nothing to hide: all keys before all columns, inside every column's window (or among the sinks), one sequence
-            const bool whole = one_seq && c0 + 127u <= t_first && c0 >= s_first &&
-                               (a.window == 0u || t_first + 127u < c0 + a.window || c0 + 128u <= s_first + a.sinks);
-            ok = __all_sync(0xffffffffu, wait(s_full, j & 1u) ? 1 : 0) != 0;
+            const bool whole = one_seq && c0 + kKeys - 1u <= t_first && c0 >= s_first &&
+                               (a.window == 0u || t_first + 127u < c0 + a.window || c0 + kKeys <= s_first + a.sinks);
+            ok = __all_sync(0xffffffffu, wait(s_full + 8u * (j & 1u), (j >> 1) & 1u) ? 1 : 0) != 0;
             if (!ok) break;
             ptx::tc_fence_after();
-            float mx = -INFINITY;
-            uint32_t r[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32(lane_base + 32u * q, r[q]);
+            uint32_t r[2][32];
+            ptx::tmem_ld_32x32(from, r[0]);
+            ptx::tmem_ld_32x32(from + 32u, r[1]);
             ptx::tmem_ld_wait();
             if (!whole) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t see = seen(c0 + 32u * q);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const uint32_t c = c0 + 32u * q + i;
-                        if (!(c - lo < span || c - s0 < sk)) r[q][i] = 0xff800000u;
-                    }
+                    for (int i = 0; i < 32; ++i) if (!(see & (1u << i))) r[q][i] = 0xff800000u;
+                }
             }
+            float top[8];                                                  // short chains
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(r[0][c]);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[q][i]));
-            mx *= mul;
+            for (int i = 8; i < 64; ++i) top[i & 7] = fmaxf(top[i & 7], __uint_as_float(r[i >> 5][i & 31]));
+            const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * mul;
             if (__any_sync(0xffffffffu, mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY))) {
                 const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
                 m = mn;
                 l *= f;
                 if (j != 0u) {
+                    ok = __all_sync(0xffffffffu, wait(pv_done, (j - 1u) & 1u) ? 1 : 0) != 0;       // the product before this one still adds to the output
+                    if (!ok) break;
+                    ptx::tc_fence_after();
 #pragma unroll 1
                     for (uint32_t d0 = 0; d0 < D; d0 += 32u) {
                         uint32_t o[32];
@@ -277,36 +331,30 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             }
             const float shift = m == -INFINITY ? 0.f : m;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t p[32];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                uint32_t p[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = fast_exp2(fmaf(__uint_as_float(r[2 * q + (i >> 4)][2 * (i & 15)]), mul, -shift));
-                    const float y = fast_exp2(fmaf(__uint_as_float(r[2 * q + (i >> 4)][2 * (i & 15) + 1]), mul, -shift));
-                    sum[(2 * i) & 3] += x;
-                    sum[(2 * i + 1) & 3] += y;
-                    const __half2 h = __floats2half2_rn(x, y);
-                    p[i] = *reinterpret_cast<const uint32_t *>(&h);
-                }
-                ptx::tmem_st_32x32(lane_base + 32u * q, p);
+            for (int i = 0; i < 32; ++i) {
+                const float x = fast_exp2(fmaf(__uint_as_float(r[i >> 4][2 * (i & 15)]), mul, -shift));
+                const float y = fast_exp2(fmaf(__uint_as_float(r[i >> 4][2 * (i & 15) + 1]), mul, -shift));
+                sum[(2 * i) & 3] += x;
+                sum[(2 * i + 1) & 3] += y;
+                const __half2 h = __floats2half2_rn(x, y);
+                p[i] = *reinterpret_cast<const uint32_t *>(&h);
             }
+            ptx::tmem_st_32x32(from, p);
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(p_full);
+            ptx::mbar_arrive(p_full + 8u * (j & 1u));
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(o_full, 0u) ? 1 : 0) != 0;
+        if (ok) ok = __all_sync(0xffffffffu, wait(pv_done, (n - 1u) & 1u) ? 1 : 0) != 0;
         if (ok) {
             ptx::tc_fence_after();
             const float inv = 1.0f / l;
             // values that were kept from the tensor cores: a column that sees one gets it
             bool flagged = false;
             const uint32_t *flags = a.v_flags + hk * (a.pitch / 64u);
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t f = key_tile(j) * 2u;
-                flagged |= flags[f] != 0u || (f + 1u < a.pitch / 64u && flags[f + 1u] != 0u);
-            }
+            for (uint32_t j = 0; j < n; ++j) flagged |= flags[key_tile(j)] != 0u;
             __half *dst = a.out + (uint64_t)hq * D * a.pitch + t;
 #pragma unroll 1
             for (uint32_t d0 = 0; d0 < D; d0 += 32u) {
@@ -315,9 +363,9 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 ptx::tmem_ld_wait();
                 if (flagged && t < a.columns) {
                     for (uint32_t j = 0; j < n; ++j) {
-                        const uint32_t c0 = key_tile(j) * 128u;
-                        for (uint32_t c = c0; c < c0 + 128u && c <= t; ++c) {
-                            if (!(c - lo < span || c - s0 < sk)) continue;
+                        const uint32_t c0 = key_tile(j) * kKeys;
+                        for (uint32_t c = c0; c < c0 + kKeys && c <= t; ++c) {
+                            if (!(seen(c) & 1u)) continue;
                             const __half *col = a.v + ((uint64_t)hk * D + d0) * a.pitch + c;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
@@ -368,13 +416,16 @@ cudaError_t window_attn_setup() {
 cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m, bool pdl, cudaStream_t s) {
     // operands for whole tiles of 128 columns (what lies behind the last column is zero, not whatever the scratch held)
     const uint32_t tiles = (a.columns + 127u) / 128u;
-    const dim3 g1(std::min(2u * tiles, a.pitch / 64u), a.h_q + 2u * a.h_kv), g2(a.h_q, tiles);
+    const uint32_t wide = std::min(2u * tiles, a.pitch / 64u), turned = a.h_q + a.h_kv;
+    // several heads per CTA (they share the angles, and one head's rows load while another's are turned) where that leaves CTAs enough
+    const uint32_t heads = std::max(1u, std::min(8u, wide * turned / 592u));
+    const dim3 g1(wide, (turned + heads - 1u) / heads + a.h_kv), g2(a.h_q, tiles);
     cudaError_t e;
     if (a.head_dim == 64u) {
-        e = launch_dep(k44_window_operands_kernel<64>, g1, dim3(256), 0, pdl, s, a);
+        e = launch_dep(k44_window_operands_kernel<64>, g1, dim3(256), 0, pdl, s, a, heads);
         if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.q, m.k, m.v, a);
     } else {
-        e = launch_dep(k44_window_operands_kernel<128>, g1, dim3(256), 0, pdl, s, a);
+        e = launch_dep(k44_window_operands_kernel<128>, g1, dim3(256), 0, pdl, s, a, heads);
         if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.q, m.k, m.v, a);
     }
     return e;
