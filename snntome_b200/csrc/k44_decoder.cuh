@@ -87,7 +87,7 @@ struct WindowAttnArgs {
     uint32_t pitch = 0, columns = 0, h_q = 0, h_kv = 0, head_dim = 0, seq_len = 0, window = 0, sinks = 0;
     unsigned long long wait_cycles = 0;
 };
-struct WindowAttnMaps { CUtensorMap q, k, v; };
+struct WindowAttnMaps { CUtensorMap q, k, v, out; };
 uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_q, uint32_t h_kv, uint32_t head_dim);
 void window_attn_place(WindowAttnArgs &a, void *scratch);
 cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m, bool pdl, cudaStream_t s);

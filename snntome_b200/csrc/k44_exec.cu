@@ -594,7 +594,8 @@ bool Executor::place_window(DeviceWave &dw) {
         return encode_map_2d(map, base, inner, outer, 64u, box_rows);
     };
     return rows(&dw.window_maps.q, a.q_rows, a.head_dim, (uint64_t)a.h_q * a.pitch, 128u) && rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 64u) &&
-           rows(&dw.window_maps.v, a.v_rows, a.pitch, (uint64_t)a.h_kv * a.head_dim, a.head_dim);
+           rows(&dw.window_maps.v, a.v_rows, a.pitch, (uint64_t)a.h_kv * a.head_dim, a.head_dim) &&
+           encode_map_2d(&dw.window_maps.out, a.out, a.pitch, (uint64_t)a.h_q * a.head_dim, 64u, a.head_dim, false);
 }
 
 bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {

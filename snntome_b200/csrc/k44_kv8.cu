@@ -7,6 +7,7 @@
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
 
+#include <algorithm>
 #include <numeric>
 
 namespace k44b {
@@ -62,17 +63,35 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // ---- filling the cache from a prompt ----------------------------------------------------------------------------------------
-// CTA = one block of 64 tokens of one sequence and head. Keys are rotated and rounded to FP16 first, then treated as the step
-// by step path treats them. HBM-bound: 4 bytes read and 2 written per pair of key and value elements.
+// CTA = one block of 64 tokens of one sequence, some of its heads one after the other. Keys are rotated and rounded to FP16 first,
+// then treated as the step by step path treats them. HBM-bound: 4 bytes read and 2 written per pair of key and value elements.
+// Keys pass through shared memory once, to be turned from channel rows to token rows: a thread owns one token and 8 rotation pairs,
+// neighbours the next pairs, so that table and codes are read and written in whole sectors and a token's elements stay in registers
+// from the rotation to the code. Values need no turning: a thread takes 8 tokens of a channel from the canvas to their codes. The
+// next head's rows load meanwhile. Columns are read from the 16-byte boundary below a sequence's first one.
 template <int D>
-__global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a) {
+__global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a, uint32_t heads) {
     dep_enter();
-    constexpr int ROW = 64 + 8;                                      // padded row of 64 tokens (halves)
+    constexpr uint32_t PER = D / 16, TOKENS = 256u / PER, ROUNDS = 64u / TOKENS, N = D / 32;   // N pieces of 8 values per thread
+    constexpr uint32_t ROW = 64 + 10;                                // 37 words: rows 8 apart, and pieces of neighbouring rows, on different banks
     __shared__ __align__(16) __half ks[D * ROW];
     __shared__ __align__(16) __half vs[D * ROW];
     __shared__ float red[2][8];
-    const uint32_t block = blockIdx.x, h = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;
+    const uint32_t block = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x, H = a.cache.h_kv;
+    const uint32_t t0 = block * kKv8Block, part = tid % PER, p0 = part * 8u, tok0 = tid / PER;
     const int2 sl = a.sequences[seq];
+    float2 cs[ROUNDS][8];
+#pragma unroll
+    for (uint32_t n = 0; n < ROUNDS; ++n) {
+        const uint32_t t = t0 + n * TOKENS + tok0;
+        const float4 *from = reinterpret_cast<const float4 *>(a.rope + (uint64_t)t * (D / 2) + p0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = t < a.seq_len ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            cs[n][2 * i] = make_float2(v.x, v.y);
+            cs[n][2 * i + 1] = make_float2(v.z, v.w);
+        }
+    }
     if (sl.x < 0) return;
     const uint32_t len = (uint32_t)sl.y;
     // a plan's tables are checked by the host; the cache's own limits are checked here as well
@@ -80,84 +99,128 @@ __global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a) 
         if (tid == 0u) atomicOr(a.status, (uint32_t)ST_BAD_INDEX);
         return;
     }
-    const uint64_t ch = (uint64_t)sl.x * a.cache.h_kv + h;
-    if (block == 0u && tid == 0u) a.cache.tail_block[ch] = (len % kKv8Block) ? (int)(len / kKv8Block) : -1;
-    const uint32_t t0 = block * kKv8Block;
+    const uint32_t h0 = blockIdx.y * heads, h1 = min(h0 + heads, H);
+    if (block == 0u && tid < h1 - h0) a.cache.tail_block[(uint64_t)sl.x * H + h0 + tid] = (len % kKv8Block) ? (int)(len / kKv8Block) : -1;
     if (t0 >= len) return;
-    const uint32_t n = min(kKv8Block, len - t0), col0 = seq * a.seq_len + t0;
-    const __half *kg = a.k + (uint64_t)h * D * a.pitch + col0, *vg = a.v + (uint64_t)h * D * a.pitch + col0;
-    if ((col0 & 7u) == 0u) {
-        for (uint32_t e = tid; e < D * 8u; e += 256u) {              // 16-byte pieces; a piece that starts inside the row ends inside it
-            const uint32_t d = e >> 3, c = (e & 7u) * 8u;
-            uint4 kk = make_uint4(0, 0, 0, 0), vv = kk;
-            if (c < n) {
-                kk = __ldg(reinterpret_cast<const uint4 *>(kg + (uint64_t)d * a.pitch + c));
-                vv = __ldg(reinterpret_cast<const uint4 *>(vg + (uint64_t)d * a.pitch + c));
+    const uint32_t n = min(kKv8Block, len - t0), col0 = seq * a.seq_len + t0, shift = col0 & 7u, base = col0 - shift, end = shift + n;
+    // piece e of a head: 8 columns of row e >> 3; with a shift, a ninth piece per row. Pieces start before column `columns`, and rows
+    // are whole multiples of 64 columns, so a piece that starts inside a row ends inside it.
+    uint4 kn[N], vn[N];
+    auto fetch = [&](uint32_t h) {
+        const __half *kg = a.k + (uint64_t)h * D * a.pitch + base, *vg = a.v + (uint64_t)h * D * a.pitch + base;
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t e = 256u * i + tid, c = (e & 7u) * 8u;
+            const uint64_t at = (uint64_t)(e >> 3) * a.pitch + c;
+            kn[i] = vn[i] = make_uint4(0, 0, 0, 0);
+            if (c < end) {
+                kn[i] = __ldg(reinterpret_cast<const uint4 *>(kg + at));
+                vn[i] = __ldg(reinterpret_cast<const uint4 *>(vg + at));
             }
-            *reinterpret_cast<uint4 *>(ks + d * ROW + c) = kk;
-            *reinterpret_cast<uint4 *>(vs + d * ROW + c) = vv;
         }
-    } else {                                                         // sequences that do not start on a 16-byte boundary
-        for (uint32_t e = tid; e < D * 64u; e += 256u) {
-            const uint32_t d = e >> 6, c = e & 63u;
-            ks[d * ROW + c] = c < n ? kg[(uint64_t)d * a.pitch + c] : __half(0.f);
-            vs[d * ROW + c] = c < n ? vg[(uint64_t)d * a.pitch + c] : __half(0.f);
+    };
+    auto put = [](__half *row, uint4 x) {
+        uint32_t *to = reinterpret_cast<uint32_t *>(row);
+        to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
+    };
+    fetch(h0);
+    for (uint32_t h = h0; h < h1; ++h) {
+        const uint64_t ch = (uint64_t)sl.x * H + h;
+        uint4 vv[N];
+        if (h != h0) __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t e = 256u * i + tid;
+            put(ks + (e >> 3) * ROW + (e & 7u) * 8u, kn[i]);
+            vv[i] = vn[i];
+            if (shift) put(vs + (e >> 3) * ROW + (e & 7u) * 8u, vn[i]);
         }
-    }
-    __syncthreads();
-    // rotate: a thread owns one token and every fourth pair
-    const uint32_t tok = tid & 63u, part = tid >> 6;
-    float kmax = 0.f, vmax = 0.f;
-    if (tok < n) {
-        const float2 *cs = a.rope + (uint64_t)(t0 + tok) * (D / 2);
-#pragma unroll 4
-        for (uint32_t p = part; p < D / 2; p += 4u) {
-            float x = __half2float(ks[p * ROW + tok]), y = __half2float(ks[(p + D / 2) * ROW + tok]);
-            rotate(x, y, __ldg(cs + p));
-            const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
-            ks[p * ROW + tok] = hx;
-            ks[(p + D / 2) * ROW + tok] = hy;
-            kmax = amax_of(amax_of(kmax, __half2float(hx)), __half2float(hy));
-            vmax = amax_of(amax_of(vmax, __half2float(vs[p * ROW + tok])), __half2float(vs[(p + D / 2) * ROW + tok]));
+        if (end > 64u && tid < D) {                                  // the ninth pieces
+            const uint64_t at = ((uint64_t)h * D + tid) * a.pitch + base + 64u;
+            put(ks + tid * ROW + 64u, __ldg(reinterpret_cast<const uint4 *>(a.k + at)));
+            put(vs + tid * ROW + 64u, __ldg(reinterpret_cast<const uint4 *>(a.v + at)));
         }
-    }
+        __syncthreads();
+        if (h + 1u < h1) fetch(h + 1u);
+        float kmax = 0.f, vmax = 0.f;
+        uint32_t lo[ROUNDS][4], hi[ROUNDS][4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-    }
-    if ((tid & 31u) == 0u) { red[0][tid >> 5] = kmax; red[1][tid >> 5] = vmax; }
-    __syncthreads();
-    if (n == kKv8Block) {                                            // a whole block: 8 bits
+        for (uint32_t r = 0; r < ROUNDS; ++r) {
+            const __half *x = ks + p0 * ROW + shift + r * TOKENS + tok0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) { kmax = fmaxf(kmax, red[0][w]); vmax = fmaxf(vmax, red[1][w]); }
-        const float ksc = scale_of(kmax), vsc = scale_of(vmax), ki = 1.0f / ksc, vi = 1.0f / vsc;
-        uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D);
-        if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block] = make_float2(ksc, vsc);
-        for (uint32_t e = tid; e < 64u * D / 16u; e += 256u) {        // 16 codes of a key: 16 dimensions of one token
-            const uint32_t t = e & 63u, d0 = (e >> 6) * 16u;
-            uint32_t w[4];
+            for (uint32_t i = 0; i < 4; ++i) {
+                float u[2], v[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __half *x = ks + (d0 + 4 * i) * ROW + t;
-                w[i] = codes4(__half2float(x[0]), __half2float(x[ROW]), __half2float(x[2 * ROW]), __half2float(x[3 * ROW]), ki);
+                for (uint32_t e = 0; e < 2; ++e) {
+                    u[e] = __half2float(x[(2 * i + e) * ROW]);
+                    v[e] = __half2float(x[(2 * i + e + D / 2) * ROW]);
+                    rotate(u[e], v[e], cs[r][2 * i + e]);
+                }
+                lo[r][i] = pack2(u[0], u[1]);
+                hi[r][i] = pack2(v[0], v[1]);
+                const float2 f = half2_of(lo[r][i]), g = half2_of(hi[r][i]);
+                kmax = amax_of(amax_of(amax_of(amax_of(kmax, f.x), f.y), g.x), g.y);
             }
-            *reinterpret_cast<uint4 *>(codes + (d0 >> 6) * 4096u + t * 64u + (d0 & 63u)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        for (uint32_t e = tid; e < 64u * D / 16u; e += 256u) {        // 16 codes of a value: 16 tokens of one dimension
-            const uint32_t d = e >> 2, c = (e & 3u) * 16u;
-            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 x = half2_of(*reinterpret_cast<const uint32_t *>(vs + d * ROW + c + 4 * i)), y = half2_of(*reinterpret_cast<const uint32_t *>(vs + d * ROW + c + 4 * i + 2));
-                w[i] = codes4(x.x, x.y, y.x, y.y, vi);
+        for (uint32_t i = 0; i < N; ++i) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(&vv[i]);
+            if (shift) {
+                const uint32_t e = 256u * i + tid;
+                const unsigned short *x = reinterpret_cast<const unsigned short *>(vs + (e >> 3) * ROW + (e & 7u) * 8u + shift);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)x[2 * j] | ((uint32_t)x[2 * j + 1] << 16);
             }
-            *reinterpret_cast<uint4 *>(codes + kKv8Block * D + d * 64u + c) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const float2 f = half2_of(w[j]); vmax = amax_of(amax_of(vmax, f.x), f.y); }
         }
-    } else {                                                         // the open block: FP16 rows; rows behind the last token stay as they were
-        __half *kt = a.cache.k_tail + ch * (kKv8Block * D), *vt = a.cache.v_tail + ch * (kKv8Block * D);
-        for (uint32_t e = tid; e < n * D; e += 256u) { const uint32_t t = e / D, d = e % D; kt[t * D + d] = ks[d * ROW + t]; }
-        for (uint32_t e = tid; e < 64u * D; e += 256u) { const uint32_t d = e >> 6, c = e & 63u; if (c < n) vt[d * 64u + c] = vs[d * ROW + c]; }
+        if (n == kKv8Block) {                                        // a whole block: 8 bits
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
+                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            }
+            if ((tid & 31u) == 0u) { red[0][tid >> 5] = kmax; red[1][tid >> 5] = vmax; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 8; ++w) { kmax = fmaxf(kmax, red[0][w]); vmax = fmaxf(vmax, red[1][w]); }
+            const float ksc = scale_of(kmax), vsc = scale_of(vmax), ki = 1.0f / ksc, vi = 1.0f / vsc;
+            uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D);
+            if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block] = make_float2(ksc, vsc);
+            auto eight = [](const uint32_t *w, float inv) {
+                const float2 x = half2_of(w[0]), y = half2_of(w[1]), z = half2_of(w[2]), q = half2_of(w[3]);
+                return make_uint2(codes4(x.x, x.y, y.x, y.y, inv), codes4(z.x, z.y, q.x, q.y, inv));
+            };
+#pragma unroll
+            for (uint32_t r = 0; r < ROUNDS; ++r) {
+                uint8_t *row = codes + (r * TOKENS + tok0) * 64u;
+                constexpr uint32_t H2 = D / 2;
+                *reinterpret_cast<uint2 *>(row + p0) = eight(lo[r], ki);
+                *reinterpret_cast<uint2 *>(row + ((p0 + H2) >> 6) * 4096u + ((p0 + H2) & 63u)) = eight(hi[r], ki);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i)
+                *reinterpret_cast<uint2 *>(codes + kKv8Block * D + (256u * i + tid) * 8u) = eight(reinterpret_cast<const uint32_t *>(&vv[i]), vi);
+        } else {                                                     // the open block: FP16 rows; rows behind the last token stay as they were
+            __half *kt = a.cache.k_tail + ch * (kKv8Block * D), *vt = a.cache.v_tail + ch * (kKv8Block * D);
+#pragma unroll
+            for (uint32_t r = 0; r < ROUNDS; ++r) {
+                const uint32_t t = r * TOKENS + tok0;
+                if (t >= n) continue;
+                *reinterpret_cast<uint4 *>(kt + t * D + p0) = make_uint4(lo[r][0], lo[r][1], lo[r][2], lo[r][3]);
+                *reinterpret_cast<uint4 *>(kt + t * D + p0 + D / 2) = make_uint4(hi[r][0], hi[r][1], hi[r][2], hi[r][3]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t e = 256u * i + tid, c = (e & 7u) * 8u;
+                if (c + 8u <= n) *reinterpret_cast<uint4 *>(vt + e * 8u) = vv[i];
+                else {
+                    const __half *x = reinterpret_cast<const __half *>(&vv[i]);
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) if (c + j < n) vt[e * 8u + j] = x[j];
+                }
+            }
+        }
     }
 }
 
@@ -812,9 +875,11 @@ cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_d
 }
 
 cudaError_t launch_kv8_fill(const Kv8FillArgs &a, bool pdl, cudaStream_t s) {
-    const dim3 grid((a.seq_len + kKv8Block - 1u) / kKv8Block, a.cache.h_kv, (a.columns + a.seq_len - 1u) / a.seq_len);
-    return a.cache.head_dim == 64u ? launch_dep(k44_kv8_fill_kernel<64>, grid, dim3(256), 0, pdl, s, a)
-                                   : launch_dep(k44_kv8_fill_kernel<128>, grid, dim3(256), 0, pdl, s, a);
+    const uint32_t blocks = (a.seq_len + kKv8Block - 1u) / kKv8Block, seqs = (a.columns + a.seq_len - 1u) / a.seq_len, H = a.cache.h_kv;
+    const uint32_t heads = std::max(1u, std::min(4u, blocks * seqs * H / 592u));
+    const dim3 grid(blocks, (H + heads - 1u) / heads, seqs);
+    return a.cache.head_dim == 64u ? launch_dep(k44_kv8_fill_kernel<64>, grid, dim3(256), 0, pdl, s, a, heads)
+                                   : launch_dep(k44_kv8_fill_kernel<128>, grid, dim3(256), 0, pdl, s, a, heads);
 }
 
 cudaError_t kv8_attn_setup() {

@@ -19,9 +19,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) != 0x7c00u; }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
-// CTA = 64 columns of a few heads of q and k, or of one head of v. Columns behind the plan's last one become zero. Values that are not finite become
-// zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the tensor cores;
-// the attention adds them to the columns that do see them.
+// CTA = 64 columns of a few heads of q and k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
+// not finite become zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
+// tensor cores; the attention adds them to the columns that do see them. The rotated q and k are rounded to FP16, the tensor cores'
+// type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16.
 template <int D>
 __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a, uint32_t heads) {
     dep_enter();
@@ -116,21 +117,26 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
 
 // ---- attention -----------------------------------------------------------------------------------------------------------------
 // Warp 0 copies (TMA), one thread of warp 1 issues the MMAs, warps 2-5 are the softmax: a thread owns one column (= TMEM lane).
-// Tensor memory: two buffers of 64 columns of scores, over whose first half the weights are written as FP16 pairs once the scores
-// are read (the A operand of the second product), and D columns of output. That is half of the SM's, so two CTAs share an SM. While
-// the softmax works on one buffer the next scores are already being made in the other, so that its warps wait for nothing of their
-// own CTA's but their own loads, and those hide behind the other CTA's exponentials: 128 x 128 of them take 1024 cycles of the SM's 16
-// per cycle, their products 256 (D = 64) — the exponentials bound this kernel, not the tensor cores. (One buffer of 128 keys per CTA:
-// 2340 cycles.)
+// Tensor memory: a buffer of 64 columns of scores, over whose first half the weights are written as FP16 pairs once the scores are
+// read (the A operand of the second product), and D columns of output. 128 x 64 exponentials take 512 cycles of the SM's 16 per
+// cycle, their products 128 (D = 64) or 256. Nothing of it overlaps within one column's chain (scores, maximum, weights, output), so
+// what counts is how many chains an SM holds: D = 64 runs four CTAs per SM (128 columns of tensor memory each, 80 registers, the
+// second half of the scores read twice, one stage of keys and values), D = 128 two, each with a second buffer in which the next
+// scores are made meanwhile. Both launches, 8192 tokens, 32 heads on 8, window 1024, D = 64: 154 us (with two stages 160, three CTAs
+// of more registers 172, two CTAs with two buffers 164, two warps to a row 180); four prompts of 1000, 32 heads on 8, D = 128: 87 us
+// (with one buffer 107). Without its exponentials the former still takes 142, without exponentials and products 128: the chain's
+// waits and reads of tensor memory bound it.
 // The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
 // exact in FP16 as weights up to 1, and the sum is kept against the same maximum.
 template <int D> struct Shape {
     static constexpr uint32_t HF = D / 64;
     static constexpr uint32_t Q_BYTES = 128u * D * 2u, K_BYTES = 64u * D * 2u, V_BYTES = K_BYTES;
-    static constexpr uint32_t STAGES = D == 64 ? 4u : 2u;
+    static constexpr uint32_t STAGES = D == 64 ? 1u : 2u, CTAS = D == 64 ? 4u : 2u, BUFFERS = D == 64 ? 1u : 2u;
+    static constexpr bool HOLD = D != 64;                        // registers for all 64 scores
+    static constexpr uint32_t O_COL = BUFFERS * 64u, TMEM_COLS = O_COL + D > 128u ? 256u : 128u;
     static constexpr uint32_t SMEM = Q_BYTES + STAGES * (K_BYTES + V_BYTES) + 1024u + 256u;
 };
-constexpr uint32_t kThreads = 192, kTmemCols = 256, kOCol = 128, kKeys = 64;
+constexpr uint32_t kThreads = 192, kKeys = 64;
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
     // K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
@@ -141,6 +147,22 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two at a time: (a.x * b + c, a.y * b + c), and sums
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // bits from .. to of a word (either may lie outside it)
 __device__ __forceinline__ uint32_t bits(int from, int to) {
     if (to < 0 || from > 31 || from > to) return 0u;
@@ -148,10 +170,11 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 2)
-k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const WindowAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, Shape<D>::CTAS)
+k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const __grid_constant__ CUtensorMap o_map, const WindowAttnArgs a) {
     using S = Shape<D>;
-    constexpr uint32_t HF = S::HF, ST = S::STAGES;
+    constexpr uint32_t HF = S::HF, ST = S::STAGES, NB = S::BUFFERS, kOCol = S::O_COL, kTmemCols = S::TMEM_COLS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_smem = base, k_smem = q_smem + S::Q_BYTES, v_smem = k_smem + ST * S::K_BYTES, ctl = v_smem + ST * S::V_BYTES;
@@ -184,13 +207,11 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
         if (ptx::mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
-        for (uint32_t it = 0;; ++it) {
-            if (ptx::mbar_try_wait(bar, parity)) return true;
-            if ((it & 31u) == 31u) {
-                if (*abort_word != 0u) return false;
-                if ((unsigned long long)(clock64() - t0) > a.wait_cycles) return false;
-            }
+        while (!ptx::mbar_try_wait_for(bar, parity, 20000u)) {
+            if (*abort_word != 0u) return false;
+            if ((unsigned long long)(clock64() - t0) > a.wait_cycles) return false;
         }
+        return true;
     };
     // ---- which tiles of keys ----
     const uint32_t hq = blockIdx.x, qt = gridDim.y - 1u - blockIdx.y, hk = hq / (a.h_q / a.h_kv);      // the longest rows first
@@ -243,27 +264,27 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         if (lane == 0) {
             constexpr uint32_t idesc_s = (1u << 4) | ((kKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
             auto scores = [&](uint32_t j) -> bool {
-                const uint32_t s = j % ST, to = tmem + (j & 1u) * kKeys;
+                const uint32_t s = j % ST, to = tmem + j % NB * kKeys;
                 if (!wait(k_full + 8u * s, (j / ST) & 1u)) return false;
                 ptx::tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < D / 16u; ++k)
                     ptx::umma_f16(to, desc_sw128(q_smem + (k >> 2) * 16384u) + (k & 3u) * 2u, desc_sw128(k_smem + s * S::K_BYTES + (k >> 2) * 8192u) + (k & 3u) * 2u, idesc_s, k != 0u ? 1u : 0u);
                 ptx::umma_commit(k_empty + 8u * s);
-                ptx::umma_commit(s_full + 8u * (j & 1u));
+                ptx::umma_commit(s_full + 8u * (j % NB));
                 return true;
             };
-            ok = wait(q_full, 0u) && scores(0u) && (n < 2u || scores(1u));
+            ok = wait(q_full, 0u) && scores(0u) && (NB == 1u || n < 2u || scores(1u));
             for (uint32_t j = 0; j < n && ok; ++j) {
                 const uint32_t s = j % ST;
-                if (!(ok = wait(v_full + 8u * s, (j / ST) & 1u) && wait(p_full + 8u * (j & 1u), (j >> 1) & 1u))) break;
+                if (!(ok = wait(v_full + 8u * s, (j / ST) & 1u) && wait(p_full + 8u * (j % NB), (j / NB) & 1u))) break;
                 ptx::tc_fence_after();
 #pragma unroll
                 for (uint32_t k = 0; k < kKeys / 16u; ++k)
-                    ptx::umma_f16_a_tmem(tmem + kOCol, tmem + (j & 1u) * kKeys + 8u * k, desc_sw128(v_smem + s * S::V_BYTES) + k * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
+                    ptx::umma_f16_a_tmem(tmem + kOCol, tmem + j % NB * kKeys + 8u * k, desc_sw128(v_smem + s * S::V_BYTES) + k * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
                 ptx::umma_commit(v_empty + 8u * s);
                 ptx::umma_commit(pv_done);
-                if (j + 2u < n) ok = scores(j + 2u);                        // over the weights that the product before it has read
+                if (j + NB < n) ok = scores(j + NB);                        // over the weights that the product before it has read
             }
             if (!ok) {
                 if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_MMA);
@@ -285,31 +306,50 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         };
         float m = -INFINITY, l = 0.f;                                     // maximum that the weights are kept against (scaled), their sum
         for (uint32_t j = 0; j < n && ok; ++j) {
-            const uint32_t c0 = key_tile(j) * kKeys, from = lane_base + (j & 1u) * kKeys;
+            const uint32_t c0 = key_tile(j) * kKeys, from = lane_base + j % NB * kKeys;
             // nothing to hide: all keys before all columns, inside every column's window (or among the sinks), one sequence
             const bool whole = one_seq && c0 + kKeys - 1u <= t_first && c0 >= s_first &&
                                (a.window == 0u || t_first + 127u < c0 + a.window || c0 + kKeys <= s_first + a.sinks);
-            ok = __all_sync(0xffffffffu, wait(s_full + 8u * (j & 1u), (j >> 1) & 1u) ? 1 : 0) != 0;
+            ok = __all_sync(0xffffffffu, wait(s_full + 8u * (j % NB), (j / NB) & 1u) ? 1 : 0) != 0;
             if (!ok) break;
             ptx::tc_fence_after();
-            uint32_t r[2][32];
-            ptx::tmem_ld_32x32(from, r[0]);
-            ptx::tmem_ld_32x32(from + 32u, r[1]);
-            ptx::tmem_ld_wait();
-            if (!whole) {
+            uint32_t r[32], r2[S::HOLD ? 32 : 1];                              // scores of the first 32 keys, and, where registers allow, of the others
+            // Of 32 columns and 32 keys on an edge most see all or nothing: those need no mask, these no exponentials.
+            const uint32_t see0 = whole ? ~0u : seen(c0), see1 = whole ? ~0u : seen(c0 + 32u);
+            const bool any0 = whole || __any_sync(0xffffffffu, see0 != 0u), any1 = whole || __any_sync(0xffffffffu, see1 != 0u);
+            const bool all0 = whole || __all_sync(0xffffffffu, see0 == ~0u), all1 = whole || __all_sync(0xffffffffu, see1 == ~0u);
+            auto hide = [&](uint32_t (&x)[32], uint32_t see) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t see = seen(c0 + 32u * q);
+                for (int i = 0; i < 32; ++i) if (!(see & (1u << i))) x[i] = 0xff800000u;
+            };
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // short chains
+            auto largest = [&](const uint32_t (&x)[32]) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) if (!(see & (1u << i))) r[q][i] = 0xff800000u;
+                for (int i = 0; i < 16; ++i) top[i & 3] = max3(top[i & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 16]));
+            };
+            if constexpr (!S::HOLD) {
+                if (any1) {
+                    ptx::tmem_ld_32x32(from + 32u, r);
+                    ptx::tmem_ld_wait();
+                    if (!all1) hide(r, see1);
+                    largest(r);
                 }
+                if (any0) {
+                    ptx::tmem_ld_32x32(from, r);
+                    ptx::tmem_ld_wait();
+                }
+            } else {
+                ptx::tmem_ld_32x32(from, r);
+                ptx::tmem_ld_32x32(from + 32u, r2);
+                ptx::tmem_ld_wait();
+                if (!all1) hide(r2, see1);
+                if (any1) largest(r2);
             }
-            float top[8];                                                  // short chains
-#pragma unroll
-            for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(r[0][c]);
-#pragma unroll
-            for (int i = 8; i < 64; ++i) top[i & 7] = fmaxf(top[i & 7], __uint_as_float(r[i >> 5][i & 31]));
-            const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7]))) * mul;
+            if (any0) {
+                if (!all0) hide(r, see0);
+                largest(r);
+            }
+            const float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]) * mul;
             if (__any_sync(0xffffffffu, mx > m + 8.0f || (m == -INFINITY && mx != -INFINITY))) {
                 const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
                 m = mn;
@@ -330,22 +370,37 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 }
             }
             const float shift = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t p[32];
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            auto weights = [&](const uint32_t (&x)[32], bool any, uint32_t to) {
+                uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float x = fast_exp2(fmaf(__uint_as_float(r[i >> 4][2 * (i & 15)]), mul, -shift));
-                const float y = fast_exp2(fmaf(__uint_as_float(r[i >> 4][2 * (i & 15) + 1]), mul, -shift));
-                sum[(2 * i) & 3] += x;
-                sum[(2 * i + 1) & 3] += y;
-                const __half2 h = __floats2half2_rn(x, y);
-                p[i] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-            ptx::tmem_st_32x32(from, p);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                for (int i = 0; i < 16; ++i) p[i] = 0u;
+                if (any) {
+                    const float2 mul2 = make_float2(mul, mul), shift2 = make_float2(-shift, -shift);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), mul2, shift2);
+                        e.x = fast_exp2(e.x); e.y = fast_exp2(e.y);
+                        sum[i & 1] = add2(sum[i & 1], e);
+                        const __half2 h = __floats2half2_rn(e.x, e.y);
+                        p[i] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                }
+                ptx::tmem_st_32x16(to, p);
+            };
+            weights(r, any0, from);                                        // over scores that have been read: those of 32 .. 63 are still there
+            if constexpr (!S::HOLD) {
+                if (any1) {
+                    ptx::tmem_ld_32x32(from + 32u, r);
+                    ptx::tmem_ld_wait();
+                    if (!all1) hide(r, see1);
+                }
+                weights(r, any1, from + 16u);
+            } else weights(r2, any1, from + 16u);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             ptx::tmem_st_wait();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(p_full + 8u * (j & 1u));
+            ptx::mbar_arrive(p_full + 8u * (j % NB));
         }
         if (ok) ok = __all_sync(0xffffffffu, wait(pv_done, (n - 1u) & 1u) ? 1 : 0) != 0;
         if (ok) {
@@ -355,7 +410,12 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
             bool flagged = false;
             const uint32_t *flags = a.v_flags + hk * (a.pitch / 64u);
             for (uint32_t j = 0; j < n; ++j) flagged |= flags[key_tile(j)] != 0u;
-            __half *dst = a.out + (uint64_t)hq * D * a.pitch + t;
+            // Rows of the output are columns of the canvas: 2 bytes per lane and dimension, 128 stores of 64 bytes each per warp, which took
+            // 4500 cycles per item (D = 128). Whole tiles go through the shared memory that held q and out with tensor copies instead.
+            const bool tile = t_first + 128u <= a.columns;
+            __half *const out_s = reinterpret_cast<__half *>(smem_raw + (q_smem - ptx::smem_addr(smem_raw)));      // [half of the columns][dimension][64]
+            __half *dst = tile ? out_s + (row >> 6) * (D * 64u) + (row & 63u) : a.out + (uint64_t)hq * D * a.pitch + t;
+            const uint64_t step = tile ? 64u : a.pitch;
 #pragma unroll 1
             for (uint32_t d0 = 0; d0 < D; d0 += 32u) {
                 uint32_t o[32];
@@ -377,7 +437,16 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                 }
                 if (t < a.columns) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) dst[(uint64_t)(d0 + i) * a.pitch] = __float2half_rn(__uint_as_float(o[i]) * inv);
+                    for (int i = 0; i < 32; ++i) dst[(uint64_t)(d0 + i) * step] = __float2half_rn(__uint_as_float(o[i]) * inv);
+                }
+            }
+            if (tile) {
+                ptx::fence_proxy_async();
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (threadIdx.x == 64u) {
+                    for (uint32_t f = 0; f < 2u; ++f) ptx::tma_store_2d(&o_map, (int32_t)(t_first + 64u * f), (int32_t)(hq * D), q_smem + f * (D * 128u));
+                    ptx::bulk_commit_group();
+                    ptx::bulk_wait_group<0>();
                 }
             }
         } else if (lane == 0) {
@@ -423,10 +492,10 @@ cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m,
     cudaError_t e;
     if (a.head_dim == 64u) {
         e = launch_dep(k44_window_operands_kernel<64>, g1, dim3(256), 0, pdl, s, a, heads);
-        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.q, m.k, m.v, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.q, m.k, m.v, m.out, a);
     } else {
         e = launch_dep(k44_window_operands_kernel<128>, g1, dim3(256), 0, pdl, s, a, heads);
-        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.q, m.k, m.v, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.q, m.k, m.v, m.out, a);
     }
     return e;
 }
