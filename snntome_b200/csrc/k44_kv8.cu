@@ -39,9 +39,9 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 cs) {
 }
 
 // ---- 8 bits -------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float finite_abs(float x) { return fminf(fabsf(x), 65504.0f); }     // NaN -> 65504: see amax_of
-// largest magnitude of the numbers among (m, x); a NaN does not count
-__device__ __forceinline__ float amax_of(float m, float x) { return x != x ? m : fmaxf(m, finite_abs(x)); }
+// largest magnitudes so far, two at a time; the maximum of a number and a NaN is the number
+__device__ __forceinline__ __half2 amax_of(__half2 m, uint32_t two) { return __hmax2(m, __habs2(*reinterpret_cast<const __half2 *>(&two))); }
+__device__ __forceinline__ float amax_of(__half2 m) { const float2 f = __half22float2(m); return fminf(fmaxf(f.x, f.y), 65504.0f); }
 __device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(fmaxf(amax, 5.9604644775390625e-8f), 448.0f); }
 // four values -> four codes, the first in the lowest byte; the conversion saturates at +-448
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
@@ -63,35 +63,26 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // ---- filling the cache from a prompt ----------------------------------------------------------------------------------------
-// CTA = one block of 64 tokens of one sequence, some of its heads one after the other. Keys are rotated and rounded to FP16 first,
-// then treated as the step by step path treats them. HBM-bound: 4 bytes read and 2 written per pair of key and value elements.
-// Keys pass through shared memory once, to be turned from channel rows to token rows: a thread owns one token and 8 rotation pairs,
-// neighbours the next pairs, so that table and codes are read and written in whole sectors and a token's elements stay in registers
-// from the rotation to the code. Values need no turning: a thread takes 8 tokens of a channel from the canvas to their codes. The
-// next head's rows load meanwhile. Columns are read from the 16-byte boundary below a sequence's first one.
+// CTA = the keys or the values of one block of 64 tokens of one sequence, some of its heads one after the other. Keys are rotated and
+// rounded to FP16 first, then treated as the step by step path treats them. HBM-bound: 4 bytes read and 2 written per pair of key and
+// value elements. Keys pass through shared memory once, to be turned from channel rows to token rows: a thread owns one token and 8
+// rotation pairs, neighbours the next pairs, so that table and codes are read and written in whole sectors and a token's elements stay
+// in registers from the rotation to the code. Values need no turning: a thread takes 8 tokens of a channel from the canvas to their
+// codes. The next head's rows load meanwhile. Columns are read from the 16-byte boundary below a sequence's first one.
+// 64 prompts of up to 512 tokens, 8 heads of 64: 17.5 us for 50 MB. Keys and values in one CTA 20.7 (123 registers, half as many
+// CTAs); without heads in a row 25 (each CTA waits for its length, rows and angles in turn), with 2 or 3 18 to 19, with 8 20 (too
+// few CTAs). What is left is those waits of the first CTAs and the last ones' uneven end; HBM is at a fifth while it runs.
 template <int D>
-__global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a, uint32_t heads) {
+__global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(const Kv8FillArgs a, uint32_t heads) {
     dep_enter();
-    constexpr uint32_t PER = D / 16, TOKENS = 256u / PER, ROUNDS = 64u / TOKENS, N = D / 32;   // N pieces of 8 values per thread
+    constexpr uint32_t PER = D / 16, TOKENS = 256u / PER, ROUNDS = 64u / TOKENS, N = D / 32;   // N pieces of 8 elements per thread
     constexpr uint32_t ROW = 64 + 10;                                // 37 words: rows 8 apart, and pieces of neighbouring rows, on different banks
-    __shared__ __align__(16) __half ks[D * ROW];
-    __shared__ __align__(16) __half vs[D * ROW];
-    __shared__ float red[2][8];
+    __shared__ __align__(16) __half xs[D * ROW];
+    __shared__ float red[8];
     const uint32_t block = blockIdx.x, seq = blockIdx.z, tid = threadIdx.x, H = a.cache.h_kv;
-    const uint32_t t0 = block * kKv8Block, part = tid % PER, p0 = part * 8u, tok0 = tid / PER;
+    const uint32_t t0 = block * kKv8Block, part = tid % PER, p0 = part * 8u, tok0 = tid / PER, groups = gridDim.y / 2u;
+    const bool is_k = blockIdx.y < groups;
     const int2 sl = a.sequences[seq];
-    float2 cs[ROUNDS][8];
-#pragma unroll
-    for (uint32_t n = 0; n < ROUNDS; ++n) {
-        const uint32_t t = t0 + n * TOKENS + tok0;
-        const float4 *from = reinterpret_cast<const float4 *>(a.rope + (uint64_t)t * (D / 2) + p0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 v = t < a.seq_len ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            cs[n][2 * i] = make_float2(v.x, v.y);
-            cs[n][2 * i + 1] = make_float2(v.z, v.w);
-        }
-    }
     if (sl.x < 0) return;
     const uint32_t len = (uint32_t)sl.y;
     // a plan's tables are checked by the host; the cache's own limits are checked here as well
@@ -99,125 +90,143 @@ __global__ void __launch_bounds__(256) k44_kv8_fill_kernel(const Kv8FillArgs a, 
         if (tid == 0u) atomicOr(a.status, (uint32_t)ST_BAD_INDEX);
         return;
     }
-    const uint32_t h0 = blockIdx.y * heads, h1 = min(h0 + heads, H);
-    if (block == 0u && tid < h1 - h0) a.cache.tail_block[(uint64_t)sl.x * H + h0 + tid] = (len % kKv8Block) ? (int)(len / kKv8Block) : -1;
+    const uint32_t h0 = (is_k ? blockIdx.y : blockIdx.y - groups) * heads, h1 = min(h0 + heads, H);
+    if (is_k && block == 0u && tid < h1 - h0) a.cache.tail_block[(uint64_t)sl.x * H + h0 + tid] = (len % kKv8Block) ? (int)(len / kKv8Block) : -1;
     if (t0 >= len) return;
     const uint32_t n = min(kKv8Block, len - t0), col0 = seq * a.seq_len + t0, shift = col0 & 7u, base = col0 - shift, end = shift + n;
+    const __half *rows = (is_k ? a.k : a.v) + base;
     // piece e of a head: 8 columns of row e >> 3; with a shift, a ninth piece per row. Pieces start before column `columns`, and rows
     // are whole multiples of 64 columns, so a piece that starts inside a row ends inside it.
-    uint4 kn[N], vn[N];
+    uint4 next[N], ninth = make_uint4(0, 0, 0, 0);
     auto fetch = [&](uint32_t h) {
-        const __half *kg = a.k + (uint64_t)h * D * a.pitch + base, *vg = a.v + (uint64_t)h * D * a.pitch + base;
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
             const uint32_t e = 256u * i + tid, c = (e & 7u) * 8u;
-            const uint64_t at = (uint64_t)(e >> 3) * a.pitch + c;
-            kn[i] = vn[i] = make_uint4(0, 0, 0, 0);
-            if (c < end) {
-                kn[i] = __ldg(reinterpret_cast<const uint4 *>(kg + at));
-                vn[i] = __ldg(reinterpret_cast<const uint4 *>(vg + at));
-            }
+            next[i] = c < end ? __ldg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + (e >> 3)) * a.pitch + c)) : make_uint4(0, 0, 0, 0);
         }
+        if (end > 64u && tid < D) ninth = __ldg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + tid) * a.pitch + 64u));
     };
-    auto put = [](__half *row, uint4 x) {
-        uint32_t *to = reinterpret_cast<uint32_t *>(row);
+    auto stage = [&](uint32_t row, uint32_t c, uint4 x) {
+        uint32_t *to = reinterpret_cast<uint32_t *>(xs + row * ROW + c);
         to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
     };
-    fetch(h0);
-    for (uint32_t h = h0; h < h1; ++h) {
-        const uint64_t ch = (uint64_t)sl.x * H + h;
-        uint4 vv[N];
-        if (h != h0) __syncthreads();
+    auto stage_all = [&] {
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            const uint32_t e = 256u * i + tid;
-            put(ks + (e >> 3) * ROW + (e & 7u) * 8u, kn[i]);
-            vv[i] = vn[i];
-            if (shift) put(vs + (e >> 3) * ROW + (e & 7u) * 8u, vn[i]);
-        }
-        if (end > 64u && tid < D) {                                  // the ninth pieces
-            const uint64_t at = ((uint64_t)h * D + tid) * a.pitch + base + 64u;
-            put(ks + tid * ROW + 64u, __ldg(reinterpret_cast<const uint4 *>(a.k + at)));
-            put(vs + tid * ROW + 64u, __ldg(reinterpret_cast<const uint4 *>(a.v + at)));
-        }
+        for (uint32_t i = 0; i < N; ++i) { const uint32_t e = 256u * i + tid; stage(e >> 3, (e & 7u) * 8u, next[i]); }
+        if (end > 64u && tid < D) stage(tid, 64u, ninth);
         __syncthreads();
-        if (h + 1u < h1) fetch(h + 1u);
-        float kmax = 0.f, vmax = 0.f;
-        uint32_t lo[ROUNDS][4], hi[ROUNDS][4];
+    };
+    auto whole_max = [&](float m) {                                  // of the CTA; its barrier also ends all reading of xs
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((tid & 31u) == 0u) red[tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+        return m;
+    };
+    auto eight = [](const uint32_t *w, float inv) {
+        const float2 x = half2_of(w[0]), y = half2_of(w[1]), z = half2_of(w[2]), q = half2_of(w[3]);
+        return make_uint2(codes4(x.x, x.y, y.x, y.y, inv), codes4(z.x, z.y, q.x, q.y, inv));
+    };
+    fetch(h0);
+    if (is_k) {
+        float2 cs[ROUNDS][8];
 #pragma unroll
         for (uint32_t r = 0; r < ROUNDS; ++r) {
-            const __half *x = ks + p0 * ROW + shift + r * TOKENS + tok0;
+            const uint32_t t = t0 + r * TOKENS + tok0;
+            const float4 *from = reinterpret_cast<const float4 *>(a.rope + (uint64_t)t * (D / 2) + p0);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                float u[2], v[2];
-#pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) {
-                    u[e] = __half2float(x[(2 * i + e) * ROW]);
-                    v[e] = __half2float(x[(2 * i + e + D / 2) * ROW]);
-                    rotate(u[e], v[e], cs[r][2 * i + e]);
-                }
-                lo[r][i] = pack2(u[0], u[1]);
-                hi[r][i] = pack2(v[0], v[1]);
-                const float2 f = half2_of(lo[r][i]), g = half2_of(hi[r][i]);
-                kmax = amax_of(amax_of(amax_of(amax_of(kmax, f.x), f.y), g.x), g.y);
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = t < a.seq_len ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                cs[r][2 * i] = make_float2(v.x, v.y);
+                cs[r][2 * i + 1] = make_float2(v.z, v.w);
             }
         }
+        for (uint32_t h = h0; h < h1; ++h) {
+            const uint64_t ch = (uint64_t)sl.x * H + h;
+            if (h != h0) __syncthreads();
+            stage_all();
+            if (h + 1u < h1) fetch(h + 1u);
+            __half2 amax = __float2half2_rn(0.f);
+            uint32_t lo[ROUNDS][4], hi[ROUNDS][4];
+#pragma unroll
+            for (uint32_t r = 0; r < ROUNDS; ++r) {
+                const __half *x = xs + p0 * ROW + shift + r * TOKENS + tok0;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    float u[2], v[2];
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        u[e] = __half2float(x[(2 * i + e) * ROW]);
+                        v[e] = __half2float(x[(2 * i + e + D / 2) * ROW]);
+                        rotate(u[e], v[e], cs[r][2 * i + e]);
+                    }
+                    lo[r][i] = pack2(u[0], u[1]);
+                    hi[r][i] = pack2(v[0], v[1]);
+                    amax = amax_of(amax_of(amax, lo[r][i]), hi[r][i]);
+                }
+            }
+            if (n == kKv8Block) {                                    // a whole block: 8 bits
+                const float scale = scale_of(whole_max(amax_of(amax))), inv = 1.0f / scale;
+                uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D);
+                if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block].x = scale;
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; ++r) {
+                    uint8_t *row = codes + (r * TOKENS + tok0) * 64u;
+                    const uint32_t p1 = p0 + D / 2;
+                    *reinterpret_cast<uint2 *>(row + p0) = eight(lo[r], inv);
+                    *reinterpret_cast<uint2 *>(row + (p1 >> 6) * 4096u + (p1 & 63u)) = eight(hi[r], inv);
+                }
+            } else {                                                 // the open block: FP16 rows; rows behind the last token stay as they were
+                __half *tail = a.cache.k_tail + ch * (kKv8Block * D);
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; ++r) {
+                    const uint32_t t = r * TOKENS + tok0;
+                    if (t >= n) continue;
+                    *reinterpret_cast<uint4 *>(tail + t * D + p0) = make_uint4(lo[r][0], lo[r][1], lo[r][2], lo[r][3]);
+                    *reinterpret_cast<uint4 *>(tail + t * D + p0 + D / 2) = make_uint4(hi[r][0], hi[r][1], hi[r][2], hi[r][3]);
+                }
+            }
+        }
+        return;
+    }
+    for (uint32_t h = h0; h < h1; ++h) {
+        const uint64_t ch = (uint64_t)sl.x * H + h;
+        uint4 x[N];
+        if (h != h0) __syncthreads();
+        if (shift) stage_all();
+        __half2 amax = __float2half2_rn(0.f);
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
-            uint32_t *w = reinterpret_cast<uint32_t *>(&vv[i]);
+            uint32_t *w = reinterpret_cast<uint32_t *>(&x[i]);
+            x[i] = next[i];
             if (shift) {
                 const uint32_t e = 256u * i + tid;
-                const unsigned short *x = reinterpret_cast<const unsigned short *>(vs + (e >> 3) * ROW + (e & 7u) * 8u + shift);
+                const unsigned short *from = reinterpret_cast<const unsigned short *>(xs + (e >> 3) * ROW + (e & 7u) * 8u + shift);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)x[2 * j] | ((uint32_t)x[2 * j + 1] << 16);
+                for (int j = 0; j < 4; ++j) w[j] = (uint32_t)from[2 * j] | ((uint32_t)from[2 * j + 1] << 16);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { const float2 f = half2_of(w[j]); vmax = amax_of(amax_of(vmax, f.x), f.y); }
+            for (int j = 0; j < 4; ++j) amax = amax_of(amax, w[j]);
         }
-        if (n == kKv8Block) {                                        // a whole block: 8 bits
+        if (h + 1u < h1) fetch(h + 1u);
+        if (n == kKv8Block) {
+            const float scale = scale_of(whole_max(amax_of(amax))), inv = 1.0f / scale;
+            uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D) + kKv8Block * D;
+            if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block].y = scale;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-            }
-            if ((tid & 31u) == 0u) { red[0][tid >> 5] = kmax; red[1][tid >> 5] = vmax; }
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 8; ++w) { kmax = fmaxf(kmax, red[0][w]); vmax = fmaxf(vmax, red[1][w]); }
-            const float ksc = scale_of(kmax), vsc = scale_of(vmax), ki = 1.0f / ksc, vi = 1.0f / vsc;
-            uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D);
-            if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block] = make_float2(ksc, vsc);
-            auto eight = [](const uint32_t *w, float inv) {
-                const float2 x = half2_of(w[0]), y = half2_of(w[1]), z = half2_of(w[2]), q = half2_of(w[3]);
-                return make_uint2(codes4(x.x, x.y, y.x, y.y, inv), codes4(z.x, z.y, q.x, q.y, inv));
-            };
-#pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; ++r) {
-                uint8_t *row = codes + (r * TOKENS + tok0) * 64u;
-                constexpr uint32_t H2 = D / 2;
-                *reinterpret_cast<uint2 *>(row + p0) = eight(lo[r], ki);
-                *reinterpret_cast<uint2 *>(row + ((p0 + H2) >> 6) * 4096u + ((p0 + H2) & 63u)) = eight(hi[r], ki);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i)
-                *reinterpret_cast<uint2 *>(codes + kKv8Block * D + (256u * i + tid) * 8u) = eight(reinterpret_cast<const uint32_t *>(&vv[i]), vi);
-        } else {                                                     // the open block: FP16 rows; rows behind the last token stay as they were
-            __half *kt = a.cache.k_tail + ch * (kKv8Block * D), *vt = a.cache.v_tail + ch * (kKv8Block * D);
-#pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; ++r) {
-                const uint32_t t = r * TOKENS + tok0;
-                if (t >= n) continue;
-                *reinterpret_cast<uint4 *>(kt + t * D + p0) = make_uint4(lo[r][0], lo[r][1], lo[r][2], lo[r][3]);
-                *reinterpret_cast<uint4 *>(kt + t * D + p0 + D / 2) = make_uint4(hi[r][0], hi[r][1], hi[r][2], hi[r][3]);
-            }
+            for (uint32_t i = 0; i < N; ++i) *reinterpret_cast<uint2 *>(codes + (256u * i + tid) * 8u) = eight(reinterpret_cast<const uint32_t *>(&x[i]), inv);
+        } else {
+            __half *tail = a.cache.v_tail + ch * (kKv8Block * D);
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) {
                 const uint32_t e = 256u * i + tid, c = (e & 7u) * 8u;
-                if (c + 8u <= n) *reinterpret_cast<uint4 *>(vt + e * 8u) = vv[i];
+                if (c + 8u <= n) *reinterpret_cast<uint4 *>(tail + e * 8u) = x[i];
                 else {
-                    const __half *x = reinterpret_cast<const __half *>(&vv[i]);
+                    const __half *one = reinterpret_cast<const __half *>(&x[i]);
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j) if (c + j < n) vt[e * 8u + j] = x[j];
+                    for (uint32_t j = 0; j < 8; ++j) if (c + j < n) tail[e * 8u + j] = one[j];
                 }
             }
         }
@@ -398,15 +407,16 @@ __global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs 
     if (rebuild)
 #pragma unroll
         for (int i = 0; i < N; ++i) piece[i] = reinterpret_cast<const uint4 *>(tail)[32 * i + lane];
-    float mx = 0.f;
+    __half2 amax = __float2half2_rn(0.f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {                                              // the new token's row (keys) or column (values)
         const uint32_t at = (32u * i + lane) * 8u;
         if (is_k) { if (at / D == kKv8Block - 1u) piece[i] = *reinterpret_cast<const uint4 *>(x + at % D); }
         else if ((at & 63u) == 56u) piece[i].w = (piece[i].w & 0xffffu) | ((uint32_t)__half_as_ushort(x[at >> 6]) << 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { const float2 f = half2_of(word(piece[i], e)); mx = amax_of(amax_of(mx, f.x), f.y); }
+        for (int e = 0; e < 4; ++e) amax = amax_of(amax, word(piece[i], e));
     }
+    float mx = amax_of(amax);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float scale = scale_of(mx), inv = 1.0f / scale;
@@ -876,8 +886,8 @@ cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_d
 
 cudaError_t launch_kv8_fill(const Kv8FillArgs &a, bool pdl, cudaStream_t s) {
     const uint32_t blocks = (a.seq_len + kKv8Block - 1u) / kKv8Block, seqs = (a.columns + a.seq_len - 1u) / a.seq_len, H = a.cache.h_kv;
-    const uint32_t heads = std::max(1u, std::min(4u, blocks * seqs * H / 592u));
-    const dim3 grid(blocks, (H + heads - 1u) / heads, seqs);
+    const uint32_t heads = std::max(1u, std::min(4u, 2u * blocks * seqs * H / 1184u));
+    const dim3 grid(blocks, 2u * ((H + heads - 1u) / heads), seqs);
     return a.cache.head_dim == 64u ? launch_dep(k44_kv8_fill_kernel<64>, grid, dim3(256), 0, pdl, s, a, heads)
                                    : launch_dep(k44_kv8_fill_kernel<128>, grid, dim3(256), 0, pdl, s, a, heads);
 }
