@@ -11,7 +11,7 @@ enum DecoderKind : int { AUX_WINDOW_ATTN = 13, AUX_KV8_FILL = 14, AUX_KV8_ATTN =
 // ---- rotary table ------------------------------------------------------------------------------------------------------
 // (cos, sin) of position * frequency for every position and rotation pair, [positions][head_dim / 2]. Angles are formed and
 // reduced in 64 bits: a 32-bit angle at position 16000 is off by up to 1e-3, more than the rounding of an FP16 result.
-cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_dim, double theta, bool llama3, cudaStream_t s);
+cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_dim, double theta, bool llama3, bool pairs_first, cudaStream_t s);
 
 // ---- 8-bit cache ---------------------------------------------------------------------------------------------------------
 // Blocks of 64 tokens of one column (sequence) and head. Keys and values of a block lie side by side as e4m3 codes, each with
@@ -78,17 +78,17 @@ uint64_t kv8_attn_partial_bytes(uint32_t num_sms, uint32_t group, uint32_t head_
 struct WindowAttnArgs {
     const __half *q = nullptr, *k = nullptr, *v = nullptr;
     __half *out = nullptr;
-    // rotated and re-laid operands: q [h_q][pitch][head_dim], k [h_kv][pitch][head_dim], v [h_kv * head_dim][pitch] with
+    // re-laid operands: rotated k [h_kv][pitch][head_dim], v [h_kv * head_dim][pitch] with
     // non-finite values replaced by zero, and per (head, 64 columns) whether there were any
-    __half *q_rows = nullptr, *k_rows = nullptr, *v_rows = nullptr;
+    __half *k_rows = nullptr, *v_rows = nullptr;
     uint32_t *v_flags = nullptr;
-    const float2 *rope = nullptr;
+    const float2 *rope = nullptr, *rope_pairs = nullptr;       // [position][pair], [pair][position]: `positions` of them
     uint32_t *status = nullptr;
-    uint32_t pitch = 0, columns = 0, h_q = 0, h_kv = 0, head_dim = 0, seq_len = 0, window = 0, sinks = 0;
+    uint32_t pitch = 0, columns = 0, h_q = 0, h_kv = 0, head_dim = 0, seq_len = 0, window = 0, sinks = 0, positions = 0;
     unsigned long long wait_cycles = 0;
 };
-struct WindowAttnMaps { CUtensorMap q, k, v, out; };
-uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_q, uint32_t h_kv, uint32_t head_dim);
+struct WindowAttnMaps { CUtensorMap k, v, out; };
+uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_kv, uint32_t head_dim);
 void window_attn_place(WindowAttnArgs &a, void *scratch);
 cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m, bool pdl, cudaStream_t s);
 cudaError_t window_attn_setup();

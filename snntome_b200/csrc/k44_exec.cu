@@ -551,13 +551,13 @@ bool Executor::set_sequences(const int32_t *slots, const int32_t *lengths, uint3
     return true;
 }
 
-// A table of at least `positions` positions; tables live as long as the plan, so that earlier commands keep theirs.
-const float2 *Executor::rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions) {
+// A table [position][pair] of at least `positions` positions, or [pair][position] of exactly as many; tables live as long as the plan, so that earlier commands keep theirs.
+const float2 *Executor::rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions, bool pairs_first) {
     for (const auto &t : rope_tables_)
-        if (t.theta == theta && t.llama3 == llama3 && t.head_dim == head_dim && t.positions >= positions) return t.d;
-    RopeTable t{theta, llama3, head_dim, positions, nullptr};
+        if (t.theta == theta && t.llama3 == llama3 && t.head_dim == head_dim && t.pairs_first == pairs_first && (pairs_first ? t.positions == positions : t.positions >= positions)) return t.d;
+    RopeTable t{theta, llama3, pairs_first, head_dim, positions, nullptr};
     if (!check(cudaMalloc(&t.d, (size_t)positions * (head_dim / 2u) * sizeof(float2)), "rotary table allocation")) return nullptr;
-    if (!check(launch_rope_table(t.d, positions, head_dim, (double)theta, llama3, nullptr), "rotary table") || !check(cudaDeviceSynchronize(), "rotary table")) { cudaFree(t.d); return nullptr; }
+    if (!check(launch_rope_table(t.d, positions, head_dim, (double)theta, llama3, pairs_first, nullptr), "rotary table") || !check(cudaDeviceSynchronize(), "rotary table")) { cudaFree(t.d); return nullptr; }
     rope_tables_.push_back(t);
     return t.d;
 }
@@ -593,7 +593,7 @@ bool Executor::place_window(DeviceWave &dw) {
     auto rows = [&](CUtensorMap *map, void *base, uint64_t inner, uint64_t outer, uint32_t box_rows) {
         return encode_map_2d(map, base, inner, outer, 64u, box_rows);
     };
-    return rows(&dw.window_maps.q, a.q_rows, a.head_dim, (uint64_t)a.h_q * a.pitch, 128u) && rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 64u) &&
+    return rows(&dw.window_maps.k, a.k_rows, a.head_dim, (uint64_t)a.h_kv * a.pitch, 64u) &&
            rows(&dw.window_maps.v, a.v_rows, a.pitch, (uint64_t)a.h_kv * a.head_dim, a.head_dim) &&
            encode_map_2d(&dw.window_maps.out, a.out, a.pitch, (uint64_t)a.h_q * a.head_dim, 64u, a.head_dim, false);
 }
@@ -633,9 +633,11 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         a.q = canvas_ + w.src_off; a.k = canvas_ + w.src2_off; a.v = canvas_ + w.src3_off; a.out = canvas_ + w.y_off;
         a.pitch = pitch_; a.columns = columns_; a.h_q = w.h_q; a.h_kv = w.h_kv; a.head_dim = w.head_dim; a.seq_len = w.seq_len;
         a.window = w.window; a.sinks = w.sinks; a.status = d_status_; a.wait_cycles = wait_cycles;
-        if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, std::min(w.seq_len, columns_)))) return false;
+        a.positions = std::min(w.seq_len, columns_);
+        if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, a.positions)) ||
+            !(a.rope_pairs = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, a.positions, true))) return false;
         if (!check(window_attn_setup(), "kernel attribute setup")) return false;
-        const uint64_t need = window_attn_scratch_bytes(pitch_, w.h_q, w.h_kv, w.head_dim);
+        const uint64_t need = window_attn_scratch_bytes(pitch_, w.h_kv, w.head_dim);
         const bool grown = need > window_bytes_;
         if (!reserve(d_window_, window_bytes_, need, "attention scratch allocation")) return false;
         if (grown)

@@ -135,7 +135,7 @@ class Executor {
     bool encode_map_2d(CUtensorMap *map, void *base, uint64_t inner, uint64_t rows, uint32_t box_cols, uint32_t box_rows, bool swizzle128 = true);
     bool upload_out_maps(DeviceWave &dw, void *const *peer_canvases, uint32_t n);
     bool reserve_scratch(size_t tiles);
-    const float2 *rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions);
+    const float2 *rope_table(float theta, bool llama3, uint32_t head_dim, uint32_t positions, bool pairs_first = false);
     bool place_window(DeviceWave &dw);
     bool reserve(void *&p, uint64_t &have, uint64_t need, const char *what);
     bool device_memory(const void *p, const char *what);
@@ -174,7 +174,7 @@ class Executor {
     float *d_decode_partial_ = nullptr;   // per-chunk partial attention results, shared by all decode-attention commands
     size_t decode_partial_bytes_ = 0;
     // decoder operators: tables and scratch shared by all commands of the plan (they run one after the other)
-    struct RopeTable { float theta; bool llama3; uint32_t head_dim, positions; float2 *d; };
+    struct RopeTable { float theta; bool llama3, pairs_first; uint32_t head_dim, positions; float2 *d; };
     std::vector<RopeTable> rope_tables_;
     int *d_positions_ = nullptr;
     int2 *d_sequences_ = nullptr;

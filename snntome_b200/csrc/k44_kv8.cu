@@ -16,7 +16,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- rotary table ---------------------------------------------------------------------------------------------------------
-__global__ void k44_rope_table_kernel(float2 *table, uint32_t positions, uint32_t half, double theta, int llama3) {
+__global__ void k44_rope_table_kernel(float2 *table, uint32_t positions, uint32_t half, double theta, int llama3, int pairs_first) {
     const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= (uint64_t)positions * half) return;
     const uint32_t pos = (uint32_t)(i / half), p = (uint32_t)(i % half);
@@ -28,7 +28,7 @@ __global__ void k44_rope_table_kernel(float2 *table, uint32_t positions, uint32_
     }
     double s, c;
     sincos((double)pos * f, &s, &c);
-    table[i] = make_float2((float)c, (float)s);
+    table[pairs_first ? (uint64_t)p * positions + pos : i] = make_float2((float)c, (float)s);
 }
 
 // one rotation, each product and sum rounded by itself: the same bits wherever a key is rotated
@@ -878,9 +878,9 @@ template <int D, bool WIDE> cudaError_t attn_launch(const Kv8AttnArgs &a, uint32
 
 }  // namespace
 
-cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_dim, double theta, bool llama3, cudaStream_t s) {
+cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_dim, double theta, bool llama3, bool pairs_first, cudaStream_t s) {
     const uint64_t n = (uint64_t)positions * (head_dim / 2u);
-    k44_rope_table_kernel<<<(uint32_t)((n + 255u) / 256u), 256, 0, s>>>(table, positions, head_dim / 2u, theta, llama3 ? 1 : 0);
+    k44_rope_table_kernel<<<(uint32_t)((n + 255u) / 256u), 256, 0, s>>>(table, positions, head_dim / 2u, theta, llama3 ? 1 : 0, pairs_first ? 1 : 0);
     return cudaGetLastError();
 }
 

@@ -4,9 +4,10 @@
 //   visible(t, c):  s0 <= c <= t  and  (window == 0  or  c > t - window  or  c < s0 + sinks),   s0 = first column of t's sequence
 //   o_t = sum_c softmax_c(q_t . k_c / sqrt(D)) v_c
 //
-// Two launches. The first rotates q and k and lays them out token by token (the rows a tensor-core operand wants), and copies v;
-// q, k and v on the canvas stay as they are. The second is the attention: a CTA owns 128 columns of one query head and walks
-// the tiles of 64 keys that any of its columns sees — hidden tiles are never read. Tiles are cut at multiples of 64 canvas
+// Two launches. The first rotates k and lays it out token by token (the rows a tensor-core operand wants), and copies v; q, k and v
+// on the canvas stay as they are. The second is the attention: a CTA owns 128 columns of one query head, rotates its q on the way
+// into shared memory (in the first launch, written and read again, q cost 2 us more for four prompts of 1000) and walks the tiles
+// of 64 keys that any of its columns sees — hidden tiles are never read. Tiles are cut at multiples of 64 canvas
 // columns whatever the sequences' lengths, so that every copy is aligned; sequences that end inside a tile cost a mask.
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
@@ -19,16 +20,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) != 0x7c00u; }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
-// CTA = 64 columns of a few heads of q and k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
+// CTA = 64 columns of a few heads of k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
 // not finite become zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
-// tensor cores; the attention adds them to the columns that do see them. The rotated q and k are rounded to FP16, the tensor cores'
-// type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16.
+// tensor cores; the attention adds them to the columns that do see them. The rotated q and k, and the weights, are rounded to FP16, the
+// tensor cores' type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16.
 template <int D>
 __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a, uint32_t heads) {
-    dep_enter();
+    asm volatile("griddepcontrol.wait;" ::: "memory");              // in this order: the attention reads q before it waits itself
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int ROW = 64 + 2;                                     // 33 words: pairs 8 rows apart fall on different banks
     __shared__ __align__(16) __half xs[D * ROW];
-    const uint32_t tile = blockIdx.x, tid = threadIdx.x, col0 = tile * 64u, turned = (a.h_q + a.h_kv + heads - 1u) / heads;
+    const uint32_t tile = blockIdx.x, tid = threadIdx.x, col0 = tile * 64u, turned = (a.h_kv + heads - 1u) / heads;
     uint32_t h = blockIdx.y * heads;
     if (blockIdx.y >= turned) {
         h = blockIdx.y - turned;
@@ -69,18 +71,16 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
             cs[n][2 * i + 1] = make_float2(v.z, v.w);
         }
     }
-    const uint32_t h0 = h, h1 = min(h0 + heads, a.h_q + a.h_kv);
+    const uint32_t h0 = h, h1 = min(h0 + heads, a.h_kv);
     uint4 next[D / 32];                                                      // the rows of the head after this one
     auto fetch = [&](uint32_t i) {
-        const __half *src = (i < a.h_q ? a.q + (uint64_t)i * D * a.pitch : a.k + (uint64_t)(i - a.h_q) * D * a.pitch) + col0;
+        const __half *src = a.k + (uint64_t)i * D * a.pitch + col0;
 #pragma unroll
         for (int n = 0; n < D / 32; ++n) { const uint32_t e = 256u * n + tid; next[n] = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)(e >> 3) * a.pitch + (e & 7u) * 8u)); }
     };
     fetch(h0);
     for (h = h0; h < h1; ++h) {
-        const bool is_q = h < a.h_q;
-        const uint32_t head = is_q ? h : h - a.h_q;
-        __half *dst = (is_q ? a.q_rows : a.k_rows) + ((uint64_t)head * a.pitch + col0) * D;
+        __half *dst = a.k_rows + ((uint64_t)h * a.pitch + col0) * D;
         if (h != h0) __syncthreads();
 #pragma unroll
         for (int n = 0; n < D / 32; ++n) {
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
 // what counts is how many chains an SM holds: D = 64 runs four CTAs per SM (128 columns of tensor memory each, 80 registers, the
 // second half of the scores read twice, one stage of keys and values), D = 128 two, each with a second buffer in which the next
 // scores are made meanwhile. Both launches, 8192 tokens, 32 heads on 8, window 1024, D = 64: 154 us (with two stages 160, three CTAs
-// of more registers 172, two CTAs with two buffers 164, two warps to a row 180); four prompts of 1000, 32 heads on 8, D = 128: 87 us
+// of more registers 172, two CTAs with two buffers 164, two warps to a row 180); four prompts of 1000, 32 heads on 8, D = 128: 85 us
 // (with one buffer 107). Without its exponentials the former still takes 142, without exponentials and products 128: the chain's
 // waits and reads of tensor memory bound it.
 // The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
@@ -171,7 +171,7 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, Shape<D>::CTAS)
-k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                        const __grid_constant__ CUtensorMap o_map, const WindowAttnArgs a) {
     using S = Shape<D>;
     constexpr uint32_t HF = S::HF, ST = S::STAGES, NB = S::BUFFERS, kOCol = S::O_COL, kTmemCols = S::TMEM_COLS;
@@ -185,7 +185,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(q_full, 1);
+        ptx::mbar_init(q_full, 128);
         for (uint32_t s = 0; s < ST; ++s) {
             ptx::mbar_init(k_full + 8u * s, 1); ptx::mbar_init(k_empty + 8u * s, 1);
             ptx::mbar_init(v_full + 8u * s, 1); ptx::mbar_init(v_empty + 8u * s, 1);
@@ -203,7 +203,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    dep_enter();
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
         if (ptx::mbar_try_wait(bar, parity)) return true;
         const long long t0 = clock64();
@@ -213,9 +212,55 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
         }
         return true;
     };
-    // ---- which tiles of keys ----
     const uint32_t hq = blockIdx.x, qt = gridDim.y - 1u - blockIdx.y, hk = hq / (a.h_q / a.h_kv);      // the longest rows first
-    const uint32_t t_first = qt * 128u, t_last = min(t_first + 127u, a.columns - 1u);
+    const uint32_t t_first = qt * 128u;
+    // ---- q, rotated, as the rows of the first product's A operand ----
+    // A thread owns two neighbouring columns and every other group of 8 rotation pairs, so that a warp reads whole lines of the canvas.
+    // The launch of the operands starts this one once what came before it is done, so q is there before the wait below.
+    if (warp >= 2u) {
+        const uint32_t row = (warp & 1u) * 64u + 2u * lane, t = t_first + row;
+        const bool live0 = t < a.columns, live1 = t + 1u < a.columns;
+        const __half *q = a.q + (uint64_t)hq * D * a.pitch + t;
+        const float2 *r0 = a.rope_pairs + (live0 ? t % a.seq_len : 0u), *r1 = a.rope_pairs + (live1 ? (t + 1u) % a.seq_len : 0u);
+#pragma unroll
+        for (uint32_t p0 = (warp & 2u) * 4u; p0 < D / 2u; p0 += 16u) {
+            uint32_t x[8], y[8];
+            float2 c0[8], c1[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = live0 ? __ldg(reinterpret_cast<const uint32_t *>(q + (uint64_t)(p0 + i) * a.pitch)) : 0u;
+                y[i] = live0 ? __ldg(reinterpret_cast<const uint32_t *>(q + (uint64_t)(p0 + i + D / 2u) * a.pitch)) : 0u;
+                c0[i] = __ldg(r0 + (uint64_t)(p0 + i) * a.positions);
+                c1[i] = __ldg(r1 + (uint64_t)(p0 + i) * a.positions);
+            }
+            uint32_t w[4][4];                                               // [column, half][pairs]
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 u[2], v[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[2 * i + e])), g = __half22float2(*reinterpret_cast<const __half2 *>(&y[2 * i + e]));
+                    const float2 a0 = c0[2 * i + e], a1 = c1[2 * i + e];
+                    u[e] = make_float2(f.x * a0.x - g.x * a0.y, f.y * a1.x - g.y * a1.y);
+                    v[e] = make_float2(f.x * a0.y + g.x * a0.x, f.y * a1.y + g.y * a1.x);
+                }
+                const __half2 h[4] = {__floats2half2_rn(u[0].x, u[1].x), __floats2half2_rn(v[0].x, v[1].x), __floats2half2_rn(u[0].y, u[1].y), __floats2half2_rn(v[0].y, v[1].y)};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k][i] = k < 2 || live1 ? *reinterpret_cast<const uint32_t *>(&h[k]) : 0u;
+            }
+            uint8_t *rows = smem_raw + (q_smem - ptx::smem_addr(smem_raw));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {                                   // 16 bytes each, in the 128-byte swizzle
+                const uint32_t n = row + (k >> 1), d = p0 + (k & 1) * (D / 2u);
+                *reinterpret_cast<uint4 *>(rows + (d >> 6) * 16384u + n * 128u + ((((d & 63u) >> 3) ^ (n & 7u)) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+            }
+        }
+        ptx::fence_proxy_async();
+        ptx::mbar_arrive(q_full);
+    }
+    dep_enter();
+    // ---- which tiles of keys ----
+    const uint32_t t_last = min(t_first + 127u, a.columns - 1u);
     const uint32_t s_first = t_first / a.seq_len * a.seq_len;                       // start of the first column's sequence
     const bool one_seq = t_last - s_first < a.seq_len;
     uint32_t lo_first = s_first;
@@ -230,8 +275,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
     if (warp == 0) {
         if (lane == 0) {
             const uint64_t keep = ptx::policy_evict_last();
-            ptx::mbar_arrive_expect_tx(q_full, S::Q_BYTES);
-            for (uint32_t f = 0; f < HF; ++f) ptx::tma_load_2d(q_smem + f * 16384u, &q_map, (int32_t)(64u * f), (int32_t)(hq * a.pitch + t_first), q_full, keep);
             uint32_t k_issued = 0, v_issued = 0;
             for (uint32_t j = 0; j < n; ++j) {
                 const uint32_t s = j % ST, ph = (j / ST) & 1u, c0 = key_tile(j) * kKeys;
@@ -254,7 +297,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
                     while (!done && (unsigned long long)(clock64() - t0) < a.wait_cycles) done = ptx::mbar_try_wait(bar, parity);
                     if (!done) atomicOr(a.status, (uint32_t)ST_TIMEOUT_DRAIN);
                 };
-                drain(q_full, 0u);
                 for (uint32_t i = k_issued > ST ? k_issued - ST : 0u; i < k_issued; ++i) drain(k_full + 8u * (i % ST), (i / ST) & 1u);
                 for (uint32_t i = v_issued > ST ? v_issued - ST : 0u; i < v_issued; ++i) drain(v_full + 8u * (i % ST), (i / ST) & 1u);
             }
@@ -462,15 +504,14 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_c
 
 }  // namespace
 
-uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_q, uint32_t h_kv, uint32_t head_dim) {
+uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_kv, uint32_t head_dim) {
     const uint64_t row = (uint64_t)pitch * head_dim * 2u;
-    return kv8_align(h_q * row) + 2u * kv8_align(h_kv * row) + kv8_align((uint64_t)h_kv * (pitch / 64u) * 4u);
+    return 2u * kv8_align(h_kv * row) + kv8_align((uint64_t)h_kv * (pitch / 64u) * 4u);
 }
 
 void window_attn_place(WindowAttnArgs &a, void *scratch) {
     const uint64_t row = (uint64_t)a.pitch * a.head_dim * 2u;
     uint8_t *p = (uint8_t *)scratch;
-    a.q_rows = (__half *)p; p += kv8_align(a.h_q * row);
     a.k_rows = (__half *)p; p += kv8_align(a.h_kv * row);
     a.v_rows = (__half *)p; p += kv8_align(a.h_kv * row);
     a.v_flags = (uint32_t *)p;
@@ -485,17 +526,17 @@ cudaError_t window_attn_setup() {
 cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m, bool pdl, cudaStream_t s) {
     // operands for whole tiles of 128 columns (what lies behind the last column is zero, not whatever the scratch held)
     const uint32_t tiles = (a.columns + 127u) / 128u;
-    const uint32_t wide = std::min(2u * tiles, a.pitch / 64u), turned = a.h_q + a.h_kv;
+    const uint32_t wide = std::min(2u * tiles, a.pitch / 64u), turned = a.h_kv;
     // several heads per CTA (they share the angles, and one head's rows load while another's are turned) where that leaves CTAs enough
     const uint32_t heads = std::max(1u, std::min(8u, wide * turned / 592u));
     const dim3 g1(wide, (turned + heads - 1u) / heads + a.h_kv), g2(a.h_q, tiles);
     cudaError_t e;
     if (a.head_dim == 64u) {
         e = launch_dep(k44_window_operands_kernel<64>, g1, dim3(256), 0, pdl, s, a, heads);
-        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.q, m.k, m.v, m.out, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<64>, g2, dim3(kThreads), Shape<64>::SMEM, pdl, s, m.k, m.v, m.out, a);
     } else {
         e = launch_dep(k44_window_operands_kernel<128>, g1, dim3(256), 0, pdl, s, a, heads);
-        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.q, m.k, m.v, m.out, a);
+        if (e == cudaSuccess) e = launch_dep(k44_window_attn_kernel<128>, g2, dim3(kThreads), Shape<128>::SMEM, pdl, s, m.k, m.v, m.out, a);
     }
     return e;
 }
