@@ -190,8 +190,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             ptx::mbar_init(k_full + 8u * s, 1); ptx::mbar_init(k_empty + 8u * s, 1);
             ptx::mbar_init(v_full + 8u * s, 1); ptx::mbar_init(v_empty + 8u * s, 1);
         }
-        for (uint32_t b = 0; b < 2u; ++b) { ptx::mbar_init(s_full + 8u * b, 1); ptx::mbar_init(p_full + 8u * b, 128); }
-        ptx::mbar_init(pv_done, 1);
+        for (uint32_t b = 0; b < 2u; ++b) { ptx::mbar_init(s_full + 8u * b, 1); ptx::mbar_init(p_full + 8u * b, 128); ptx::mbar_init(pv_done + 8u * b, 1); }
         *abort_word = 0;
         ptx::fence_mbar_init();
     }
@@ -325,7 +324,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                 for (uint32_t k = 0; k < kKeys / 16u; ++k)
                     ptx::umma_f16_a_tmem(tmem + kOCol, tmem + j % NB * kKeys + 8u * k, desc_sw128(v_smem + s * S::V_BYTES) + k * 2u, idesc_o, (j != 0u || k != 0u) ? 1u : 0u);
                 ptx::umma_commit(v_empty + 8u * s);
-                ptx::umma_commit(pv_done);
+                ptx::umma_commit(pv_done + 8u * (j & 1u));
                 if (j + NB < n) ok = scores(j + NB);                        // over the weights that the product before it has read
             }
             if (!ok) {
@@ -346,6 +345,10 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             const int at = (int)c0;
             return bits((int)lo - at, (int)t - at) | bits((int)s0 - at, (int)(s0 + sk) - 1 - at);
         };
+        // Scores j are made after the product j - BUFFERS, so a warp that has seen them knows of the products up to j - 2 at least. A parity tells
+        // two phases apart: with one barrier for all products, a warp ahead of the others would take the end of product j - 3 for
+        // that of j - 1. So odd and even products have a barrier each.
+        auto product_done = [&](uint32_t j) -> bool { return wait(pv_done + 8u * (j & 1u), (j >> 1) & 1u); };
         float m = -INFINITY, l = 0.f;                                     // maximum that the weights are kept against (scaled), their sum
         for (uint32_t j = 0; j < n && ok; ++j) {
             const uint32_t c0 = key_tile(j) * kKeys, from = lane_base + j % NB * kKeys;
@@ -397,7 +400,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                 m = mn;
                 l *= f;
                 if (j != 0u) {
-                    ok = __all_sync(0xffffffffu, wait(pv_done, (j - 1u) & 1u) ? 1 : 0) != 0;       // the product before this one still adds to the output
+                    ok = __all_sync(0xffffffffu, product_done(j - 1u) ? 1 : 0) != 0;       // the product before this one still adds to the output
                     if (!ok) break;
                     ptx::tc_fence_after();
 #pragma unroll 1
@@ -444,7 +447,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             ptx::tc_fence_before();
             ptx::mbar_arrive(p_full + 8u * (j % NB));
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(pv_done, (n - 1u) & 1u) ? 1 : 0) != 0;
+        if (ok) ok = __all_sync(0xffffffffu, product_done(n - 1u) ? 1 : 0) != 0;
         if (ok) {
             ptx::tc_fence_after();
             const float inv = 1.0f / l;

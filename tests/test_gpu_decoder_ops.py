@@ -95,6 +95,33 @@ def test_window_attention_hidden_columns_do_not_count():
     plan.close()
 
 
+@pytest.mark.parametrize("dim,window", [(64, 0), (128, 0), (64, 300), (128, 300)])
+def test_window_attention_with_every_multiprocessor_busy(dim, window):
+    """Long rows on more CTAs than fit at once, whose warps drift apart: many runs, one result, and the right one."""
+    import torch
+    h_q, h_kv, seq, columns = 32, 8, 1000, 3000
+    rng = np.random.default_rng(dim + window)
+    pitch, rq, rk = pitch_of(columns), h_q * dim, h_kv * dim
+    body = rng.normal(0, 1, (rq + 2 * rk, pitch)).astype(np.float16)
+    plan, canvas = make_plan(body, rq, columns)
+    o = (rq + 2 * rk) * pitch
+    plan.add_window_attn(0, rq * pitch, (rq + rk) * pitch, o, h_q, h_kv, dim, seq, window=window, sinks=4, theta=THETA)
+    plan.execute()
+    first = canvas.clone()
+    for i in range(30):
+        canvas[o:] = float(SENTINEL)
+        plan.execute() if i % 2 else plan.execute_graph()
+        assert torch.equal(canvas.view(torch.int16), first.view(torch.int16)), "every run gives the same bits"
+    assert plan.status() == 0
+    got = read(canvas, pitch)
+    x = body[:, :columns].astype(np.float64)
+    for h in (0, 13, 31):
+        k = h // (h_q // h_kv)
+        want, bound = D.window_attention(x[h * dim: (h + 1) * dim], x[rq + k * dim: rq + (k + 1) * dim], x[rq + rk + k * dim: rq + rk + (k + 1) * dim], 1, 1, seq, columns, window, 4, THETA)
+        within(got[rq + 2 * rk + h * dim: rq + 2 * rk + (h + 1) * dim, :columns], want, bound, f"window attention, head {h}")
+    plan.close()
+
+
 # ---- the cache ---------------------------------------------------------------------------------------------------------------------
 def cache_arrays(cache):
     import torch
