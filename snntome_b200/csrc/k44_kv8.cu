@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
             const float4 *from = reinterpret_cast<const float4 *>(a.rope + (uint64_t)t * (D / 2) + p0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 v = t < a.seq_len ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 v = t < len ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);       // the table may end with the cache
                 cs[r][2 * i] = make_float2(v.x, v.y);
                 cs[r][2 * i + 1] = make_float2(v.z, v.w);
             }

@@ -209,6 +209,33 @@ def test_fill(h_kv, dim, seq, frames, columns, max_seq):
     plan.close()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seq,max_seq", [(133, 133), (141, 133), (203, 135), (134, 1000)])
+def test_fill_from_any_column(dim, seq, max_seq):
+    """Sequences that start on odd columns, and plans whose sequences are longer than the cache, leave the bits that aligned ones leave."""
+    import torch
+    h_kv, lengths = 3, np.array([133, 64, 128, 1, 70, 131, 0, 40, 129], dtype=np.int32)
+    rng = np.random.default_rng(seq + dim)
+    rk, frames = h_kv * dim, len(lengths)
+    data = rng.normal(0, 1, (2 * rk, frames, 133)).astype(np.float16)
+    got = []
+    for s in (192, seq):
+        pitch = pitch_of(frames * s)
+        body = np.full((2 * rk, pitch), np.nan, dtype=np.float16)          # what lies between the sequences must not matter
+        for f, n in enumerate(lengths):
+            body[:, f * s: f * s + n] = data[:, f, :n]
+        cache = KV8Cache(frames, h_kv, dim, max_seq)
+        cache.storage.fill_(77)
+        plan, canvas = make_plan(body, 0, frames * s)
+        plan.add_kv8_fill(cache, 0, rk * pitch, s, theta=THETA)
+        plan.set_sequences(np.arange(frames, dtype=np.int32)[::-1].copy(), lengths)
+        plan.execute()
+        assert plan.status() == 0
+        got.append(cache.storage.clone())
+        plan.close()
+    assert torch.equal(got[0], got[1])
+
+
 class Decoder:
     """A plan with one kv8_attn over a cache that random tokens fill step by step, and the oracle's view of it."""
 
