@@ -568,6 +568,7 @@ bool Executor::reserve(void *&p, uint64_t &have, uint64_t need, const char *what
     void *grown = nullptr;
     if (!check(cudaDeviceSynchronize(), "synchronise") || !check(cudaMalloc(&grown, need), what)) return false;
     if (!check(cudaMemset(grown, 0, need), what) || !check(cudaDeviceSynchronize(), what)) { cudaFree(grown); return false; }
+    drop_graph();                                   // one captured before holds the old buffer
     cudaFree(p);
     p = grown; have = need;
     return true;
@@ -669,12 +670,12 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         if (!(a.positions = positions_ptr())) return false;
         if (!(a.rope = rope_table(w.rope_theta, w.llama3_scaling, w.head_dim, w.max_seq))) return false;
         if (!check(kv8_attn_setup(), "kernel attribute setup")) return false;
-        if (!reserve(d_kv8_partial_, kv8_partial_bytes_, kv8_attn_partial_bytes((uint32_t)num_sms_, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") ||
-            !reserve(d_kv8_frag_, kv8_frag_bytes_, kv8_attn_frag_bytes(columns_, w.h_kv, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") ||
-            !reserve(d_kv8_counters_, kv8_counter_bytes_, (uint64_t)columns_ * w.h_kv * sizeof(uint32_t), "attention scratch allocation")) return false;
+        const bool enough = reserve(d_kv8_partial_, kv8_partial_bytes_, kv8_attn_partial_bytes((uint32_t)num_sms_, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") &&
+                            reserve(d_kv8_frag_, kv8_frag_bytes_, kv8_attn_frag_bytes(columns_, w.h_kv, w.h_q / w.h_kv, w.head_dim), "attention scratch allocation") &&
+                            reserve(d_kv8_counters_, kv8_counter_bytes_, (uint64_t)columns_ * w.h_kv * sizeof(uint32_t), "attention scratch allocation");
         a.partial = (float *)d_kv8_partial_; a.counters = (uint32_t *)d_kv8_counters_; a.q_frag = (uint4 *)d_kv8_frag_;
         for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_KV8_ATTN) { o.kv8.partial = a.partial; o.kv8.counters = a.counters; o.kv8.q_frag = a.q_frag; }
-        return true;
+        return enough;                                                  // where only some have grown, the commands before this one have them now
     }
     case AUX_LOGPROBS: {
         if (!w.cout || w.cout > kLogprobMaxRows || !inside(w.src_off, w.cout)) return bad("the logits leave the canvas, or have too many rows");
