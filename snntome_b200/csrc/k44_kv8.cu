@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs 
     if (is_q) for (uint32_t r = rows + tid; r < (uint32_t)ROWS; r += 256u)      // rows of the operand without a head
 #pragma unroll
         for (int c = 0; c < 8; ++c) xs[c * PAD + r] = __half(0.f);
+    if (is_q && lane == 0u && col < C) a.counters[ch] = 0u;                    // of the parts that have arrived; a run that gave up leaves some
     if (is_q && head == 0u && lane == 0u && col < C && pos < 0 && a.positions[col] >= 0) atomicOr(a.status, (uint32_t)ST_BAD_INDEX);
     __syncthreads();
     if (pos < 0) return;
@@ -803,7 +804,6 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
             before = __shfl_sync(0xffffffffu, before, 0);
             if (before + n_units == sn.units) {                                  // all parts are there
                 __threadfence();
-                if (lane == 0u) a.counters[ch] = 0u;
                 const uint32_t w0 = worker_of(seg0), n = worker_of(seg0 + sn.units - 1u) - w0 + 1u;
                 auto part = [&](uint32_t i) -> const float * { return a.partial + ((uint64_t)(w0 + i) * 2u + (share(w0 + i) >= seg0 ? 0u : 1u)) * (GP * PROW); };
                 // a lane takes four dimensions of a row, the parts in their order, four of them in flight (short code: it is fetched cold)
