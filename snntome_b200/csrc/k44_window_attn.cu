@@ -448,6 +448,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             ptx::mbar_arrive(p_full + 8u * (j % NB));
         }
         if (ok) ok = __all_sync(0xffffffffu, product_done(n - 1u) ? 1 : 0) != 0;
+        const bool tile = t_first + 128u <= a.columns;
         if (ok) {
             ptx::tc_fence_after();
             const float inv = 1.0f / l;
@@ -457,7 +458,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             for (uint32_t j = 0; j < n; ++j) flagged |= flags[key_tile(j)] != 0u;
             // Rows of the output are columns of the canvas: 2 bytes per lane and dimension, 128 stores of 64 bytes each per warp, which took
             // 4500 cycles per item (D = 128). Whole tiles go through the shared memory that held q and out with tensor copies instead.
-            const bool tile = t_first + 128u <= a.columns;
             __half *const out_s = reinterpret_cast<__half *>(smem_raw + (q_smem - ptx::smem_addr(smem_raw)));      // [half of the columns][dimension][64]
             __half *dst = tile ? out_s + (row >> 6) * (D * 64u) + (row & 63u) : a.out + (uint64_t)hq * D * a.pitch + t;
             const uint64_t step = tile ? 64u : a.pitch;
@@ -488,15 +488,19 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             if (tile) {
                 ptx::fence_proxy_async();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (threadIdx.x == 64u) {
+                if (threadIdx.x == 64u && *abort_word == 0u) {
                     for (uint32_t f = 0; f < 2u; ++f) ptx::tma_store_2d(&o_map, (int32_t)(t_first + 64u * f), (int32_t)(hq * D), q_smem + f * (D * 128u));
                     ptx::bulk_commit_group();
                     ptx::bulk_wait_group<0>();
                 }
             }
-        } else if (lane == 0) {
-            if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_EPILOGUE);
-            *abort_word = 1u;
+        } else {
+            if (lane == 0) {
+                if (*abort_word == 0u) atomicOr(a.status, (uint32_t)ST_TIMEOUT_EPILOGUE);
+                *abort_word = 1u;
+            }
+            __syncwarp();
+            if (tile) asm volatile("bar.arrive 1, 128;" ::: "memory");         // a warp that came through may wait for this one
         }
     }
     ptx::tc_fence_before();
