@@ -514,7 +514,7 @@ bool Executor::set_positions(const int32_t *pos, uint32_t n, cudaStream_t stream
     }
     for (const auto &o : waves_)
         if (o.is_aux && o.aux.kind == AUX_KV8_ATTN && most >= (int64_t)o.kv8.cache.max_seq) return fail("set_positions: position " + std::to_string(most) + " lies outside the cache of '" + o.name + "'");
-    if (!not_capturing(stream, "set_positions") || !positions_ptr()) return false;
+    if (!check(cudaSetDevice(device_), "cudaSetDevice") || !not_capturing(stream, "set_positions") || !positions_ptr()) return false;
     // a copy from pageable memory is staged by the runtime before the call returns
     return check(cudaMemcpyAsync(d_positions_, pos, (size_t)n * sizeof(int32_t), cudaMemcpyHostToDevice, stream), "set_positions");
 }
@@ -543,7 +543,7 @@ bool Executor::set_sequences(const int32_t *slots, const int32_t *lengths, uint3
     std::string why;
     for (const auto &o : waves_)
         if (o.is_aux && o.aux.kind == AUX_KV8_FILL && !sequences_fit(o.fill, s, l, why)) return fail("set_sequences: '" + o.name + "': " + why);
-    if (!not_capturing(stream, "set_sequences") || !sequences_ptr()) return false;
+    if (!check(cudaSetDevice(device_), "cudaSetDevice") || !not_capturing(stream, "set_sequences") || !sequences_ptr()) return false;
     std::vector<int2> table(pitch_, make_int2(-1, 0));
     for (uint32_t i = 0; i < n; ++i) table[i] = make_int2(s[i], l[i]);
     if (!check(cudaMemcpyAsync(d_sequences_, table.data(), table.size() * sizeof(int2), cudaMemcpyHostToDevice, stream), "set_sequences")) return false;
@@ -630,6 +630,7 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
     case AUX_WINDOW_ATTN: {
         if (!w.seq_len) return bad("seq_len must not be 0");
         if ((uint64_t)w.h_q * pitch_ >= 0x7fffffffull || rk * pitch_ >= 0x7fffffffull * 64ull) return bad("too many columns");
+        if ((columns_ + 127u) / 128u > 65535u) return bad("too many columns");
         WindowAttnArgs &a = dw.window;
         a.q = canvas_ + w.src_off; a.k = canvas_ + w.src2_off; a.v = canvas_ + w.src3_off; a.out = canvas_ + w.y_off;
         a.pitch = pitch_; a.columns = columns_; a.h_q = w.h_q; a.h_kv = w.h_kv; a.head_dim = w.head_dim; a.seq_len = w.seq_len;
