@@ -58,12 +58,12 @@ __device__ __forceinline__ void add_row(const uint4 &v, const float (&base)[8], 
         __half2 h = reinterpret_cast<const __half2 *>(&v)[k];
         if (CLAMP) h = __hmax2_nan(h, least);
         const float2 x = __half22float2(h);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float t = fmaf(e ? x.y : x.x, kLog2e, -base[2 * k + e]), p = fast_exp2(t);
-            l[2 * k + e] += p;
-            w[2 * k + e] = fmaf(p, CLAMP ? t : fmaxf(t, kLeast), w[2 * k + e]);
-        }
+        float2 t = ptx::fma2(x, make_float2(kLog2e, kLog2e), make_float2(-base[2 * k], -base[2 * k + 1]));
+        const float2 p = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+        if (!CLAMP) t = make_float2(fmaxf(t.x, kLeast), fmaxf(t.y, kLeast));
+        const float2 l2 = ptx::add2(make_float2(l[2 * k], l[2 * k + 1]), p), w2 = ptx::fma2(p, t, make_float2(w[2 * k], w[2 * k + 1]));
+        l[2 * k] = l2.x; l[2 * k + 1] = l2.y;
+        w[2 * k] = w2.x; w[2 * k + 1] = w2.y;
     }
 }
 
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) k44_logprob_parts_kernel(const LogprobArg
 }
 
 // More columns: tiles of 64. A warp's groups come as tensor copies of 64 rows x 64 columns (8 KB) and are read from shared memory
-// twice (maxima, exponentials). 16 warps with one group each in flight (128256 x 1000 logits, both launches: 68 us) beat 12 with two
+// twice (maxima, exponentials). 16 warps with one group each in flight (128256 x 1000 logits, both launches: 65 us) beat 12 with two
 // (70) and 24 with one (73); held in registers, two groups per warp, the compiler spilled 600 bytes a thread (136 us).
 constexpr int kTileWarps = 16, kTileStages = 1;
 constexpr uint32_t kTileBytes = kLogprobGroup * 64u * 2u, kTileSmem = kTileWarps * kTileStages * kTileBytes + 1024u;

@@ -148,16 +148,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 // two at a time: (a.x * b + c, a.y * b + c), and sums
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)), "l"(reinterpret_cast<unsigned long long &>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long &>(d)) : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
-    return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -424,9 +414,9 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                     const float2 mul2 = make_float2(mul, mul), shift2 = make_float2(-shift, -shift);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), mul2, shift2);
+                        float2 e = ptx::fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), mul2, shift2);
                         e.x = fast_exp2(e.x); e.y = fast_exp2(e.y);
-                        sum[i & 1] = add2(sum[i & 1], e);
+                        sum[i & 1] = ptx::add2(sum[i & 1], e);
                         const __half2 h = __floats2half2_rn(e.x, e.y);
                         p[i] = *reinterpret_cast<const uint32_t *>(&h);
                     }
