@@ -6,9 +6,10 @@
 //
 // t_r is one fused multiply-add; that log2 e is a 32-bit number moves x_r by 1.3e-8 of itself, a quarter of its 32-bit rounding.
 //
-// Two launches. The first reads the logits once. A warp owns groups of 64 rows. HBM-bound for many columns: the exponentials, 16 per cycle
-// and SM, take two thirds of the time of the bytes, so that every other instruction per value counts. The group's maximum is taken on packed FP16 pairs, then every value costs one exponential against the largest value so far, without a
-// rescale of its own. It leaves (M, L, W) per chunk of rows and the maximum of every group. The second launch, one CTA per column, joins the
+// Two launches. The first reads the logits once. A warp owns groups of 64 rows. HBM-bound for many columns: the exponentials, 16 per
+// cycle and SM, take two thirds of the time of the bytes, so that every other instruction per value counts. The group's maximum is
+// taken on packed FP16 pairs, then every value costs one exponential against the largest value so far, without a rescale of its
+// own, and half a 32-bit operation each on packed pairs. It leaves (M, L, W) per chunk of rows and the maximum of every group. The second launch, one CTA per column, joins the
 // chunks and finds the alternatives exactly: ordered by (maximum, lower rows first), the first `top` of any division of the rows
 // into groups hold the `top` largest values, because the best row of each of those groups comes before every row of any other
 // group. So it goes from blocks of 512 rows to groups of 64 to rows, and reads only `top` * 64 values again.
@@ -145,7 +146,7 @@ __device__ __forceinline__ void leave_maxima(const LogprobArgs &a, const __half2
     if (col + 1u < a.columns) to[a.group_stride] = (uint16_t)order_of(u >> 16);
 }
 
-// Up to 32 columns: CG groups of 8 columns (a lane reads 16 bytes of a row), 32 / CG rows per warp load. A group's rows stay in
+// Up to 16 columns: CG groups of 8 columns (a lane reads 16 bytes of a row), 32 / CG rows per warp load. A group's rows stay in
 // registers between its maximum and its exponentials. Warp w of a chunk takes its groups w, w + 8, ...
 template <int CG>
 __global__ void __launch_bounds__(256) k44_logprob_parts_kernel(const LogprobArgs a) {
@@ -434,10 +435,10 @@ __global__ void __launch_bounds__(kFinalThreads) k44_logprob_final_kernel(const 
 
 }  // namespace
 
-// Chunks: one wave of CTAs, each with at least a group per warp. Up to 32 columns four CTAs of 8 warps fit an SM, wider tensors have
-// one of 12 warps.
+// Chunks: one wave of CTAs, each with at least a group per warp. Up to 16 columns four CTAs of 8 warps fit an SM, wider tensors have
+// one of 16 warps.
 static uint32_t chunk_groups_of(uint32_t groups, uint32_t columns, uint32_t num_sms) {
-    const bool tiles = columns > 32u;
+    const bool tiles = columns > 16u;
     const uint32_t warps = tiles ? kTileWarps : 8u, ctas = tiles ? std::max(1u, num_sms / ((columns + 63u) / 64u)) : 4u * num_sms;
     return std::max(warps, (groups + ctas - 1u) / ctas);
 }
@@ -461,12 +462,12 @@ void logprob_place(LogprobArgs &a, void *scratch, uint32_t num_sms) {
 cudaError_t logprob_setup() { return cudaFuncSetAttribute(k44_logprob_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem); }
 
 cudaError_t launch_logprobs(const LogprobArgs &a, const CUtensorMap &map, bool pdl, cudaStream_t s) {
-    // columns beyond the plan's are not read: a lane's 16 bytes are 8 columns, and few columns leave most lanes to rows
+    // Few columns: those beyond the plan's are not read, a lane's 16 bytes are 8 columns and most lanes are left to rows. 128256 rows, 20
+    // alternatives: 16 columns 14.5 us (tiles 15.2), 32 columns 17.8 (tiles 15.1), so more than 16 take tiles.
     const uint32_t cg = (a.columns + 7u) / 8u;
     cudaError_t e;
     if (cg == 1u) e = launch_dep(k44_logprob_parts_kernel<1>, dim3(1, a.chunks), dim3(256), 0, pdl, s, a);
     else if (cg == 2u) e = launch_dep(k44_logprob_parts_kernel<2>, dim3(1, a.chunks), dim3(256), 0, pdl, s, a);
-    else if (cg <= 4u) e = launch_dep(k44_logprob_parts_kernel<4>, dim3(1, a.chunks), dim3(256), 0, pdl, s, a);
     else e = launch_dep(k44_logprob_tiles_kernel, dim3((a.columns + 63u) / 64u, a.chunks), dim3(kTileWarps * 32), kTileSmem, pdl, s, map, a);
     if (e == cudaSuccess) e = launch_dep(k44_logprob_final_kernel, dim3(a.columns), dim3(kFinalThreads), 0, pdl, s, a);
     return e;

@@ -524,7 +524,8 @@ cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m,
     // operands for whole tiles of 128 columns (what lies behind the last column is zero, not whatever the scratch held)
     const uint32_t tiles = (a.columns + 127u) / 128u;
     const uint32_t wide = std::min(2u * tiles, a.pitch / 64u), turned = a.h_kv;
-    // several heads per CTA (they share the angles, and one head's rows load while another's are turned) where that leaves CTAs enough
+    // several heads per CTA (they share the angles, and one head's rows load while another's are turned) where that leaves CTAs enough:
+    // 8192 tokens, 32 heads on 32: 175 us for both launches, with one head per CTA 180
     const uint32_t heads = std::max(1u, std::min(8u, wide * turned / 592u));
     const dim3 g1(wide, (turned + heads - 1u) / heads + a.h_kv), g2(a.h_q, tiles);
     cudaError_t e;
