@@ -9,8 +9,8 @@
 // Two launches. The first reads the logits once. A warp owns groups of 64 rows. HBM-bound for many columns: the exponentials, 16 per
 // cycle and SM, take two thirds of the time of the bytes, so that every other instruction per value counts. The group's maximum is
 // taken on packed FP16 pairs, then every value costs one exponential against the largest value so far, without a rescale of its
-// own, and half a 32-bit operation each on packed pairs. It leaves (M, L, W) per chunk of rows and the maximum of every group. The second launch, one CTA per column, joins the
-// chunks and finds the alternatives exactly: ordered by (maximum, lower rows first), the first `top` of any division of the rows
+// own, and half a 32-bit operation each on packed pairs. It leaves (M, L, W) per chunk of rows and the maximum of every group. The
+// second launch, one CTA per column, joins the chunks and finds the alternatives exactly: ordered by (maximum, lower rows first), the first `top` of any division of the rows
 // into groups hold the `top` largest values, because the best row of each of those groups comes before every row of any other
 // group. So it goes from blocks of 512 rows to groups of 64 to rows, and reads only `top` * 64 values again.
 //
