@@ -417,7 +417,9 @@ static bool kv8_cache_ok(const k44b_kv8_cache *c, std::string &why) {
 
 uint64_t k44b_kv8_bytes(uint32_t columns, uint32_t h_kv, uint32_t head_dim, uint32_t max_seq) {
     if (!columns || !h_kv || !max_seq || max_seq > 0x7fffffffu || (head_dim != 64u && head_dim != 128u)) return 0;
-    if ((uint64_t)columns * h_kv > (1ull << 32)) return 0;                 // far beyond any device; keeps the products below in 64 bits
+    // far beyond any device: 2^32 blocks are 32 TiB; keeps every product and sum of the layout in 64 bits
+    const uint64_t ch = (uint64_t)columns * h_kv, blocks = ((uint64_t)max_seq + kKv8Block - 1u) / kKv8Block;
+    if (ch > (1ull << 32) || ch * blocks > (1ull << 32)) return 0;
     Kv8Cache c;
     return kv8_layout(c, nullptr, columns, h_kv, head_dim, max_seq);
 }

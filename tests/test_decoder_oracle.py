@@ -65,6 +65,14 @@ def test_cache_sizes():
             KV8Cache(*bad)
 
 
+@pytest.mark.parametrize("columns,h_kv,head_dim,max_seq", [(1 << 16, 1 << 16, 128, (1 << 31) - 1), (1 << 16, 1 << 15, 128, 1 << 24), (1 << 31, 1 << 31, 64, 1), ((1 << 32) - 1, (1 << 32) - 1, 64, 1)])
+def test_caches_whose_sizes_would_wrap_have_none(columns, h_kv, head_dim, max_seq):
+    lib = _lib.get_lib()
+    assert lib.k44b_kv8_bytes(columns, h_kv, head_dim, max_seq) == 0
+    desc = _lib.KV8CacheDesc(256, (1 << 64) - 1, columns, h_kv, head_dim, max_seq)      # never read: refused by its sizes
+    assert lib.k44b_kv8_clear(ctypes.byref(desc), None) == -1
+
+
 def test_calls_without_a_plan_or_a_cache_fail():
     lib = _lib.get_lib()
     desc = _lib.KV8CacheDesc(None, 0, 1, 1, 64, 8)
