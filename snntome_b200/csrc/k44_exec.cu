@@ -653,7 +653,7 @@ bool Executor::add_decoder(const HostWave &w, DeviceWave &dw) {
         Kv8FillArgs &a = dw.fill;
         a.cache = cache; a.k = canvas_ + w.src_off; a.v = canvas_ + w.src2_off;
         a.pitch = pitch_; a.columns = columns_; a.seq_len = w.seq_len; a.status = d_status_;
-        if ((columns_ + w.seq_len - 1u) / w.seq_len > 65535u) return bad("too many sequences");
+        if ((columns_ - 1u) / w.seq_len + 1u > 65535u) return bad("too many sequences");
         if (!(a.sequences = sequences_ptr())) return false;
         std::string why;
         if (!sequences_fit(a, h_slots_, h_lengths_, why)) return bad("the sequences set before do not fit: " + why);

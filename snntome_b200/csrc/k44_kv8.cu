@@ -888,8 +888,10 @@ cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_d
 }
 
 cudaError_t launch_kv8_fill(const Kv8FillArgs &a, bool pdl, cudaStream_t s) {
-    const uint32_t blocks = (a.seq_len + kKv8Block - 1u) / kKv8Block, seqs = (a.columns + a.seq_len - 1u) / a.seq_len, H = a.cache.h_kv;
-    const uint32_t heads = std::max(1u, std::min(4u, 2u * blocks * seqs * H / 1184u));
+    // no sequence is longer than any of these
+    const uint32_t longest = std::min(a.seq_len, std::min(a.columns, a.cache.max_seq)), H = a.cache.h_kv;
+    const uint32_t blocks = (longest + kKv8Block - 1u) / kKv8Block, seqs = (a.columns - 1u) / a.seq_len + 1u;
+    const uint32_t heads = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(4u, 2ull * blocks * seqs * H / 1184u));
     const dim3 grid(blocks, 2u * ((H + heads - 1u) / heads), seqs);
     return a.cache.head_dim == 64u ? launch_dep(k44_kv8_fill_kernel<64>, grid, dim3(256), 0, pdl, s, a, heads)
                                    : launch_dep(k44_kv8_fill_kernel<128>, grid, dim3(256), 0, pdl, s, a, heads);

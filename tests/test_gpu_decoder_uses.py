@@ -3,6 +3,7 @@ whose offsets pass 32 bits. The results are those of the plain use, bit for bit,
 import numpy as np
 import pytest
 
+from oracle import decoder as D
 from snntome_b200.native import KV8Cache, NativeError, NativePlan
 
 pytestmark = pytest.mark.gpu
@@ -171,6 +172,29 @@ def test_two_plans_take_turns_in_one_captured_graph():
     for a, b in zip(got, (pc, tc, cache.storage)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     prompt.close(), token.close()
+
+
+def test_a_sequence_may_be_all_of_the_plan():
+    """seq_len is a bound: one far beyond the plan's columns does what the columns' number does."""
+    import torch
+    got = []
+    for seq in (100, (1 << 31) - 1):
+        cache = KV8Cache(1, 2, 64, 90)
+        plan = NativePlan.create(12 * 64 * 128, 128, 100)
+        canvas = random_canvas(plan, 8 * 64, 128, 23)
+        plan.add_kv8_fill(cache, 4 * 64 * 128, 6 * 64 * 128, seq)
+        plan.add_window_attn(0, 4 * 64 * 128, 6 * 64 * 128, 8 * 64 * 128, 4, 2, 64, seq, window=(1 << 31) - 1, sinks=(1 << 31) - 1)
+        plan.set_sequences([0], [90])
+        plan.execute()
+        assert plan.status() == 0
+        # Not the same bits: a warp moves its columns' maxima together, those behind the plan's last one too, and they see other keys.
+        x = canvas.cpu().numpy().reshape(-1, 128)[:, :100]
+        y = x[: 8 * 64].astype(np.float64)
+        want, bound = D.window_attention(y[: 4 * 64], y[4 * 64: 6 * 64], y[6 * 64:], 4, 2, 100, 100, 0, 0, 10000.0)
+        assert np.all(np.abs(x[8 * 64:] - want) <= bound)
+        got.append(cache.storage.clone())
+        plan.close()
+    assert torch.equal(got[0], got[1])
 
 
 def test_cache_beyond_32_bits():
