@@ -234,11 +234,11 @@ def _build(s):
     elif case["op"] == "kv8_fill":
         cache = KV8Cache(case["columns"], case["h_kv"], case["dim"], case["max_seq"], storage=s["storage"])
         plan.add_kv8_fill(cache, s["k"], s["v"], case["seq"], theta=THETA, llama3=False)
-        plan.set_sequences(s["slots"].cpu().numpy(), s["lengths"].cpu().numpy())
+        s["sequences"] = s["slots"].cpu().numpy(), s["lengths"].cpu().numpy()          # what a scheduler has on the host
     elif case["op"] == "kv8_attn":
         cache = KV8Cache(case["columns"], case["h_kv"], case["dim"], case["max_seq"], storage=s["storage"])
         plan.add_kv8_attn(cache, s["q"], s["k"], s["v"], s["out"], case["h_q"], window=case["window"], sinks=case["sinks"], theta=THETA, llama3=False)
-        plan.set_positions(s["pos"].cpu().numpy())
+        s["positions"] = s["pos"].cpu().numpy()
     else:
         lp, ent, rows, tlp = s["out"]
         plan.add_logprobs(0, case["rows"], s["targets"], lp, ent, rows, tlp)
@@ -250,6 +250,11 @@ def _build(s):
 def run(s):
     case, op = s["case"], s["case"]["op"]
     if own:
+        # where the pass's sequences go and what its tokens' positions are come with every pass
+        if op == "kv8_fill":
+            s["plan"].set_sequences(*s["sequences"])
+        elif op == "kv8_attn":
+            s["plan"].set_positions(s["positions"])
         s["plan"].execute()
     elif op == "window_attn":
         _plain_window_attn(s)
