@@ -31,12 +31,18 @@ def visible(n_q: int, first: int, n_k: int, window: int, sinks: int) -> np.ndarr
     return see if window == 0 else see & ((c > t - window) | (c < sinks))
 
 
-def attend(q, k, v, see, score_err: float, weight_err: float = HALF16):
+def attend(q, k, v, see, score_err: float, weight_err: float = HALF16, least_weight: float = 2.0 ** -32):
     """softmax(q k^T / sqrt(d)) v over visible keys, and a bound on a kernel's error.
 
     A score that is off by at most delta_i (here score_err * sum_d |q_d k_d| / sqrt(d)) changes a weight by a factor within
     e^(+-2 delta), the second delta coming in through the sum; weights are rounded by weight_err on their way into the product (the sum
-    is taken before); the result is rounded to FP16. 2^-18 stands for 32-bit exponentials and sums."""
+    is taken before); the result is rounded to FP16. 2^-18 stands for 32-bit exponentials and sums.
+
+    `least_weight` bounds the rounding of weights too small for a relative one. A kernel holds 2^s w as FP16, w the weight relative to the
+    largest of its column so far, and FP16 numbers below 2^-14 are off by up to 2^-25: w by 2^(-25 - s). Later, larger weights only
+    shrink that, and the sum by which all is divided is at least 1 in the same units, so every value adds at most 2^(-25 - s) |v|. s is 7
+    for prompts (2^-32). For tokens against the cache it is 15, and the weight carries a factor between 1 and 2 of the values' scale:
+    the sum is at least 1/2 in those units, which makes 2^-39."""
     dim = q.shape[1]
     with np.errstate(invalid="ignore", over="ignore"):
         s = np.where(see, q @ k.T / np.sqrt(dim), -np.inf)
@@ -45,12 +51,13 @@ def attend(q, k, v, see, score_err: float, weight_err: float = HALF16):
         p = np.exp(s - s.max(axis=1, keepdims=True))
         p /= p.sum(axis=1, keepdims=True)
         o = np.zeros((q.shape[0], v.shape[1]))
-        spread = np.zeros_like(o)
+        spread, floor = np.zeros_like(o), np.zeros_like(o)
         for i in range(q.shape[0]):                     # hidden rows do not enter, whatever they hold
             rows = see[i]
             o[i] = p[i, rows] @ v[rows]
             spread[i] = p[i, rows] @ np.abs(v[rows])
-    bound = (np.expm1(2.0 * delta) + weight_err + 2.0 ** -18) * spread
+            floor[i] = least_weight * np.abs(v[rows]).sum(axis=0)
+    bound = (np.expm1(2.0 * delta) + weight_err + 2.0 ** -18) * spread + floor
     return o, bound + HALF16 * (np.abs(o) + bound) + TINY16
 
 

@@ -254,12 +254,17 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
 // values: 16 consecutive tokens of one dimension; which logical k index they stand for is free as long as the other operand
 // agrees, so codes go from shared memory to the operand registers without a shuffle: token of score tile i, column 2 j + e =
 // 16 j + 2 i + e, and the scores' accumulator layout is the second product's A operand as it stands.
-// The values' scale is folded into the exponent (p' = p * scale): p' <= 1 is what is rounded to FP16, and the sum uses p' / scale.
+// The values' scale is 2^e times a number between 1 and 2. That number is folded into the exponent (p' = p * number, and the sum uses
+// p' / number), while the accumulator is kept in units of 2^e and moves by a power of two, exactly, where a block has another e: what is
+// rounded to FP16 is a weight relative to the largest one, not to that times its block's scale, or one loud block (a value of
+// 6e4 next to values of 1) would leave nothing of the weights behind it. p' <= 1 is held as 2^15 p', so that FP16 has whole
+// precision down to 2^-29 and something down to 2^-40 of the largest weight.
 // q is split into two FP16 numbers (high and low part): with exact codes the scores are then as good as in 32 bits. With up to 8
 // heads the low parts are rows 8 to 15 of the operand, which would be empty, and cost nothing.
 // Measured, both launches: 48 columns at up to 8190 positions, 32 heads on 8 of 128 dimensions: 78 to 80 us for 348 MB (4.4 TB/s; the
 // same without the products: what bounds it is bytes in flight and the last warps' end); 64 columns at 511, D = 64, each
 // completing a block: 24 us; 64 columns at up to 16000 with a window of 1024: 28; one column at 1500: 15, a chain of latencies.
+constexpr float kWeightBits = 15.f;
 constexpr uint32_t kOpenWeight = 4;                              // an open block: one and a half times the bytes, and the work around it
 // warps per SM and granules per warp (192 KB of an SM's shared memory in all): as many warps as the registers allow
 template <int D, bool WIDE> constexpr uint32_t kWarps = WIDE || D == 128 ? 8u : 12u;
@@ -274,6 +279,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }       // -126 .. 127
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // what a column's token sees: 8-bit blocks [0, sink_blocks) and [from, open), and the open block
@@ -508,11 +514,15 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
     const float sm = rsqrtf((float)D) * kLog2e;
     uint32_t qh[R][KS][2], ql[R][KS][2];
     float sc_mul = 0.f, sc_log = 0.f, sc_inv = 0.f;
+    int sc_exp = 0;
     auto fetch_scales = [&](uint32_t first) {
         const uint32_t unit = first + lane;
         if (at.pos >= 0 && unit + 1u < at.seen.units) {
             const float2 sc = __ldg(a.cache.scales + ((uint64_t)at.col * H + at.head) * a.cache.blocks + block_of(at.seen, unit));
-            sc_mul = sc.x * sm; sc_log = log2f(sc.y); sc_inv = 1.0f / sc.y;
+            // the cache's own scales lie between 2^-33 and 2^8; others are left for the number, whose range is that of 32 bits
+            sc_exp = max(-60, min(60, (int)(__float_as_uint(sc.y) >> 23 & 255u) - 127));
+            const float number = sc.y * pow2(-sc_exp);
+            sc_mul = sc.x * sm; sc_log = log2f(number); sc_inv = 1.0f / number;
         }
     };
     auto fetch_head = [&]() {
@@ -610,6 +620,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
         const uint32_t n_units = min(sn.units - unit0, x_end - at.x);            // this warp's part of the (column, head): units start one after the other
         const bool has_open = unit0 + n_units == sn.units;
         float acc[DT][2 * R], m[R], l[R];
+        int unit = 0;                                                            // acc counts in 2^unit
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -625,7 +636,8 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
             } else mma16816(c[0], c[1], c[2], c[3], qh[0][k][0], ql[0][k][0], qh[0][k][1], ql[0][k][1], b0, b1);
         };
         // scores -> weights of one block: masked, scaled, running maximum; p (FP16 operand) and l
-        auto soften = [&](float (&s)[8][4], uint32_t t_base, uint32_t t_end, float mul, float lv, float rv, bool edge, uint32_t (&p)[R][8]) {
+        auto soften = [&](float (&s)[8][4], uint32_t t_base, uint32_t t_end, float mul, float lv, float rv, int ev, bool edge, uint32_t (&p)[R][8]) {
+            const float moved = pow2(unit - ev);                                 // both within +-60
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float mx = -INFINITY;
@@ -643,11 +655,12 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)), mul, lv);
-                const float mn = fmaxf(m[r], mx), shift = mn == -INFINITY ? 0.f : lv - mn;
-                if (__any_sync(0xffffffffu, mn != m[r])) {                        // a new maximum: what is summed so far shrinks
-                    const float back = mn == -INFINITY ? 1.f : fast_exp2(m[r] - mn);
+                const float mn = fmaxf(m[r], mx), shift = mn == -INFINITY ? 0.f : (lv - mn) + kWeightBits;
+                if (__any_sync(0xffffffffu, mn != m[r] || unit != ev)) {          // a new maximum: what is summed so far shrinks
+                    float back = mn == -INFINITY ? 1.f : fast_exp2(m[r] - mn);
                     m[r] = mn;
                     l[r] *= back;
+                    back *= moved;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) { acc[t][2 * r] *= back; acc[t][2 * r + 1] *= back; }
                 }
@@ -660,6 +673,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
                 }
                 l[r] = fmaf(sum, rv, l[r]);
             }
+            unit = ev;
         };
         auto weigh = [&](int t, uint32_t (&p)[R][8], int k, uint32_t b0, uint32_t b1) {
             float c2 = WIDE ? acc[t][2 * R - 2] : 0.f, c3 = WIDE ? acc[t][2 * R - 1] : 0.f;
@@ -672,6 +686,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
             // ---- an 8-bit block ----
             if (i0 && (i0 & 31u) == 0u) fetch_scales(unit0 + i0);
             const float mul = __shfl_sync(0xffffffffu, sc_mul, i0 & 31u), lv = __shfl_sync(0xffffffffu, sc_log, i0 & 31u), rv = __shfl_sync(0xffffffffu, sc_inv, i0 & 31u);
+            const int ev = __shfl_sync(0xffffffffu, sc_exp, i0 & 31u);
             const uint32_t t_base = block_of(sn, unit0 + i0) * kKv8Block;
             const bool edge = a.window != 0u && !(t_base + a.window > (uint32_t)pos || t_base + kKv8Block <= a.sinks);
             if (!(ok = arrived(0))) break;
@@ -696,7 +711,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
                 }
             }
             uint32_t p[R][8];
-            soften(s, t_base, t_base + kKv8Block, mul, lv, rv, edge, p);
+            soften(s, t_base, t_base + kKv8Block, mul, lv, rv, ev, edge, p);
             release(1);
             uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);                         // a hidden token's codes become 0: its NaN must not count
             if (edge) {
@@ -743,7 +758,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
                     for (int t = 0; t < 4; ++t) { const uint4 &kk = t < 2 ? k0 : k1; score(s[i], 4 * f + t, word(kk, 2 * (t & 1)), word(kk, 2 * (t & 1) + 1)); }
                 }
             uint32_t p[R][8];
-            soften(s, b * kKv8Block, (uint32_t)pos + 1u, sm, 0.f, 1.0f, true, p);
+            soften(s, b * kKv8Block, (uint32_t)pos + 1u, sm, 0.f, 1.0f, 0, true, p);
             release(2);
             ok = arrived(0) && arrived(1);
             if (!ok) break;
@@ -769,6 +784,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
         }
         if (!ok) break;
         // ---- this part is done: the output, or a part of it ----
+        const float counts = pow2(unit);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -779,7 +795,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
             for (int r = 0; r < R; ++r) {
                 const uint32_t row = g + 8u * r;
                 if (row < G) {
-                    const float inv = 1.0f / l[r];
+                    const float inv = counts / l[r];
                     __half *dst = a.out + ((uint64_t)(head * G + row) * D + 2u * j) * a.pitch + col;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
@@ -796,7 +812,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
                 const uint32_t row = g + 8u * r;
                 if (row < G) {
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) __stcg(reinterpret_cast<float2 *>(own + row * D + 8u * t + 2u * j), make_float2(acc[t][2 * r], acc[t][2 * r + 1]));
+                    for (int t = 0; t < DT; ++t) __stcg(reinterpret_cast<float2 *>(own + row * D + 8u * t + 2u * j), make_float2(acc[t][2 * r] * counts, acc[t][2 * r + 1] * counts));
                     if (j == 0u) __stcg(reinterpret_cast<float2 *>(own + GP * D + 2u * row), make_float2(m[r], l[r]));
                 }
             }

@@ -1,0 +1,61 @@
+"""The decoder operators at the ends of their numbers' ranges: weights far below the largest, scores of some tens, queries and keys whose
+rotation leaves FP16, values that are not finite. Against the 64-bit oracle, whose bounds follow from the kernels' roundings."""
+import numpy as np
+import pytest
+
+import test_gpu_decoder_ops as ops
+from oracle import decoder as D
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- weights far below the largest ---------------------------------------------------------------------------------------------------
+def blocks_of_8_bits(x):
+    """x [..., 64, dim] on the GPU -> codes and scales of the cache's format."""
+    import torch
+    scale = x.abs().amax(dim=(-2, -1)).clamp_min(2.0 ** -24) / 448.0
+    return (x / scale[..., None, None]).to(torch.float8_e4m3fn), scale
+
+
+@pytest.mark.parametrize("h_q,h_kv,dim,columns", [(8, 8, 64, 64), (16, 4, 128, 64), (16, 1, 64, 192), (16, 1, 128, 192)])
+def test_a_loud_block_leaves_the_weights_of_the_others(h_q, h_kv, dim, columns):
+    """Every fifth block holds one value of 6e4 and a token that leads by 6 to 10 nats, so that the others' weights, times their values'
+    scale, are as small as 2^-28 of that block's; a warp's share is some 17 blocks, which hold several of both kinds. Magnitudes of the
+    other blocks differ by up to 10^4."""
+    import torch
+    blocks = 30720 // (columns * h_kv)
+    pos = blocks * 64 + 20
+    d = ops.Decoder(h_q, h_kv, dim, columns, pos + 5, seed=41)
+    g = torch.Generator(device="cuda").manual_seed(42)
+    group = h_q // h_kv
+    # the same query for all heads of a column, and keys of two kinds: along it (rotated), and nothing
+    body = np.zeros((d.rq + 2 * d.rk, d.pitch), dtype=np.float16)
+    one = d.rng.normal(0, 1, (dim, columns)).astype(np.float16)
+    body[: d.rq, :columns] = np.tile(one, (h_q, 1))
+    body[d.rq + d.rk:, :columns] = d.rng.normal(0.01, 0.002, (d.rk, columns)).astype(np.float16)
+    q = D.rotated(one.astype(np.float64).T, np.full(columns, pos), ops.THETA)
+    lead = 6.0 + 4.0 * np.arange(columns) / columns
+    unit = torch.from_numpy(q * (lead * np.sqrt(dim) / (q * q).sum(axis=1))[:, None]).cuda().float()
+    v = d.cache.views()
+    for c in range(columns):
+        k = torch.zeros(h_kv, blocks + 1, 64, dim, device="cuda")
+        size = 10.0 ** -(torch.arange(blocks + 1, device="cuda") % 5).float()
+        x = (1.0 + 0.1 * torch.randn(h_kv, blocks + 1, 64, dim, generator=g, device="cuda")) * size[:, None, None]
+        k[:, ::5, 9] = unit[c]
+        x[:, ::5, 30, 7] = 6e4
+        kc, ks = blocks_of_8_bits(k)
+        xc, xs = blocks_of_8_bits(x)
+        v["codes"].view(torch.uint8)[c, :, :, 0] = kc.view(torch.uint8).unflatten(-1, (dim // 64, 64)).transpose(-3, -2).flatten(-3)
+        v["codes"].view(torch.uint8)[c, :, :, 1] = xc.view(torch.uint8).transpose(-2, -1).flatten(-2)
+        v["scales"][c, :, :, 0], v["scales"][c, :, :, 1] = ks, xs
+    v["k_tail"].zero_()
+    v["v_tail"].fill_(0.01)
+    out = d.step(np.full(columns, pos), check=False, body=body)
+    a = ops.cache_arrays(d.cache)
+    for c, h in [(0, 0), (columns // 3, h_kv // 2), (columns // 2 + 1, 0), (columns - 1, h_kv - 1)]:
+        parts = [ops.block_values(a, c, h, i, dim) for i in range(blocks)]
+        K = np.concatenate([i[0] for i in parts] + [a["k_tail"][c, h, :21].astype(np.float64)])
+        V = np.concatenate([i[1] for i in parts] + [a["v_tail"][c, h, :, :21].astype(np.float64).T])
+        want, bound = D.attend(np.repeat(q[c: c + 1], group, 0), K, V, np.ones((group, pos + 1), dtype=bool), 2.0 ** -21 + dim * 2.0 ** -23, least_weight=2.0 ** -39)
+        ops.within(out[h * group * dim: (h + 1) * group * dim, c].reshape(group, dim), want, bound, f"column {c} head {h}")
+    d.plan.close()
