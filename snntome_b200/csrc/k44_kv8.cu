@@ -519,9 +519,11 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
         const uint32_t unit = first + lane;
         if (at.pos >= 0 && unit + 1u < at.seen.units) {
             const float2 sc = __ldg(a.cache.scales + ((uint64_t)at.col * H + at.head) * a.cache.blocks + block_of(at.seen, unit));
-            // the cache's own scales lie between 2^-33 and 2^8; others are left for the number, whose range is that of 32 bits
-            sc_exp = max(-60, min(60, (int)(__float_as_uint(sc.y) >> 23 & 255u) - 127));
-            const float number = sc.y * pow2(-sc_exp);
+            // The cache's own scales lie between 2^-33 and 2^8. Larger ones are left for the number, whose range is that of 32 bits; one below
+            // 2^-60, such as the 0 of a block that nobody has written, counts as that: its values come out below 2^-51.
+            const float scale = sc.y < pow2(-60) ? pow2(-60) : sc.y;
+            sc_exp = min(60, (int)(__float_as_uint(scale) >> 23 & 255u) - 127);
+            const float number = scale * pow2(-sc_exp);
             sc_mul = sc.x * sm; sc_log = log2f(number); sc_inv = 1.0f / number;
         }
     };

@@ -59,3 +59,12 @@ def test_a_loud_block_leaves_the_weights_of_the_others(h_q, h_kv, dim, columns):
         want, bound = D.attend(np.repeat(q[c: c + 1], group, 0), K, V, np.ones((group, pos + 1), dtype=bool), 2.0 ** -21 + dim * 2.0 ** -23, least_weight=2.0 ** -39)
         ops.within(out[h * group * dim: (h + 1) * group * dim, c].reshape(group, dim), want, bound, f"column {c} head {h}")
     d.plan.close()
+
+
+@pytest.mark.parametrize("h_q,dim", [(4, 64), (16, 128)])
+def test_blocks_of_a_cleared_cache_are_zeros(h_q, dim):
+    """A code times its scale, 0 times 0: tokens that nobody appended have weights like others, and values of nothing."""
+    d = ops.Decoder(h_q, 1, dim, 3, 300, seed=9)
+    d.step([130, 64, 299])
+    d.step([131, 65, 5])
+    d.plan.close()
