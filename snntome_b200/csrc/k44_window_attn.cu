@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
 // (with one buffer 107). Without its exponentials the former still takes 142, without exponentials and products 128: the chain's
 // waits and reads of tensor memory bound it.
 // The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
-// exact in FP16 as weights up to 1, and the sum is kept against the same maximum.
+// exact in FP16 as weights up to 1, and the sum is kept against the same maximum. Weights are held times 2^7 (up to 2^15), so that FP16
+// has whole precision down to 2^-21 and something down to 2^-32 of the maximum: thousands of keys far below a first one still add up.
 template <int D> struct Shape {
     static constexpr uint32_t HF = D / 64;
     static constexpr uint32_t Q_BYTES = 128u * D * 2u, K_BYTES = 64u * D * 2u, V_BYTES = K_BYTES;
@@ -137,6 +138,7 @@ template <int D> struct Shape {
     static constexpr uint32_t SMEM = Q_BYTES + STAGES * (K_BYTES + V_BYTES) + 1024u + 256u;
 };
 constexpr uint32_t kThreads = 192, kKeys = 64;
+constexpr float kWeightBits = 7.f;
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
     // K-major rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart
@@ -404,7 +406,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                     }
                 }
             }
-            const float shift = m == -INFINITY ? 0.f : m;
+            const float shift = m == -INFINITY ? 0.f : m - kWeightBits;
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             auto weights = [&](const uint32_t (&x)[32], bool any, uint32_t to) {
                 uint32_t p[16];

@@ -68,3 +68,45 @@ def test_blocks_of_a_cleared_cache_are_zeros(h_q, dim):
     d.step([130, 64, 299])
     d.step([131, 65, 5])
     d.plan.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_key_far_above_the_others(dim):
+    """A first key that leads by 6 to 17 nats and whose value is nothing: the output is made of weights as small as 2^-24 of the largest."""
+    leads = [6.0, 9.0, 11.0, 13.0, 15.0, 17.0]
+    heads, seq = len(leads), 1500
+    rng = np.random.default_rng(dim)
+    pitch, r = ops.pitch_of(seq), heads * dim
+    body = np.zeros((3 * r, pitch), dtype=np.float16)
+    for h, lead in enumerate(leads):          # only the slowest pair, which a large base leaves where it is
+        body[h * dim + dim // 2 - 1] = np.sqrt(dim)
+        body[r + h * dim + dim // 2 - 1, 0] = lead
+    body[2 * r:] = rng.normal(1, 0.1, (r, pitch)).astype(np.float16)
+    body[2 * r:, 0] = 0
+    plan, canvas = ops.make_plan(body, r, seq)
+    plan.add_window_attn(0, r * pitch, 2 * r * pitch, 3 * r * pitch, heads, heads, dim, seq, theta=1e30)
+    plan.execute()
+    assert plan.status() == 0
+    x = body[:, :seq].astype(np.float64)
+    want, bound = D.window_attention(x[:r], x[r: 2 * r], x[2 * r:], heads, heads, seq, seq, 0, 0, 1e30)
+    ops.within(ops.read(canvas, pitch)[3 * r:, :seq], want, bound, "window attention")
+    plan.close()
+
+
+# ---- scores of some tens --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,window,size", [(64, 0, 3.0), (128, 0, 3.0), (64, 200, 4.0), (128, 77, 2.5)])
+def test_scores_of_some_tens(dim, window, size):
+    """Maxima that keep growing: queries and keys of `size`, scores of about its square."""
+    h_q, h_kv, seq, columns = 4, 2, 700, 1400
+    rng = np.random.default_rng(dim + window)
+    pitch, rq, rk = ops.pitch_of(columns), h_q * dim, h_kv * dim
+    body = rng.normal(0, 1, (rq + 2 * rk, pitch)).astype(np.float16)
+    body[: rq + rk] *= np.float16(size)
+    plan, canvas = ops.make_plan(body, rq, columns)
+    plan.add_window_attn(0, rq * pitch, (rq + rk) * pitch, (rq + 2 * rk) * pitch, h_q, h_kv, dim, seq, window=window, sinks=3, theta=ops.THETA)
+    plan.execute()
+    assert plan.status() == 0
+    x = body[:, :columns].astype(np.float64)
+    want, bound = D.window_attention(x[:rq], x[rq: rq + rk], x[rq + rk:], h_q, h_kv, seq, columns, window, 3, ops.THETA)
+    ops.within(ops.read(canvas, pitch)[rq + 2 * rk:, :columns], want, bound, "window attention")
+    plan.close()
