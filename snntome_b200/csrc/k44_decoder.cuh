@@ -11,6 +11,8 @@ enum DecoderKind : int { AUX_WINDOW_ATTN = 13, AUX_KV8_FILL = 14, AUX_KV8_ATTN =
 // ---- rotary table ------------------------------------------------------------------------------------------------------
 // (cos, sin) of position * frequency for every position and rotation pair, [positions][head_dim / 2]. Angles are formed and
 // reduced in 64 bits: a 32-bit angle at position 16000 is off by up to 1e-3, more than the rounding of an FP16 result.
+// pairs_first: [pair][position], and both times kWindowHeld: what the prompt attention's q is rotated by.
+constexpr float kWindowHeld = 0.5f;                  // the size at which the prompt attention holds rotated q and k
 cudaError_t launch_rope_table(float2 *table, uint32_t positions, uint32_t head_dim, double theta, bool llama3, bool pairs_first, cudaStream_t s);
 
 // ---- 8-bit cache ---------------------------------------------------------------------------------------------------------

@@ -28,7 +28,8 @@ __global__ void k44_rope_table_kernel(float2 *table, uint32_t positions, uint32_
     }
     double s, c;
     sincos((double)pos * f, &s, &c);
-    table[pairs_first ? (uint64_t)p * positions + pos : i] = make_float2((float)c, (float)s);
+    const float size = pairs_first ? kWindowHeld : 1.0f;
+    table[pairs_first ? (uint64_t)p * positions + pos : i] = make_float2(size * (float)c, size * (float)s);
 }
 
 // one rotation, each product and sum rounded by itself: the same bits wherever a key is rotated

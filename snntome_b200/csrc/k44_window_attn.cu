@@ -23,7 +23,8 @@ __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) !
 // CTA = 64 columns of a few heads of k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
 // not finite become zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
 // tensor cores; the attention adds them to the columns that do see them. The rotated q and k, and the weights, are rounded to FP16, the
-// tensor cores' type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16.
+// tensor cores' type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16. q and k are held at
+// half their size there: a pair of FP16 numbers may be sqrt(2) longer than the largest one, and halves are exact down to 2^-13.
 template <int D>
 __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAttnArgs a, uint32_t heads) {
     asm volatile("griddepcontrol.wait;" ::: "memory");              // in this order: the attention reads q before it waits itself
@@ -67,8 +68,8 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float4 v = col < a.columns ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            cs[n][2 * i] = make_float2(v.x, v.y);
-            cs[n][2 * i + 1] = make_float2(v.z, v.w);
+            cs[n][2 * i] = make_float2(kWindowHeld * v.x, kWindowHeld * v.y);
+            cs[n][2 * i + 1] = make_float2(kWindowHeld * v.z, kWindowHeld * v.w);
         }
     }
     const uint32_t h0 = h, h1 = min(h0 + heads, a.h_kv);
@@ -207,6 +208,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const uint32_t t_first = qt * 128u;
     // ---- q, rotated, as the rows of the first product's A operand ----
     // A thread owns two neighbouring columns and every other group of 8 rotation pairs, so that a warp reads whole lines of the canvas.
+    // The table's cosines and sines are half their size, and so is q (multiplied here instead, it cost 2 us of four prompts of 1000).
     // The launch of the operands starts this one once what came before it is done, so q is there before the wait below.
     if (warp >= 2u) {
         const uint32_t row = (warp & 1u) * 64u + 2u * lane, t = t_first + row;
@@ -328,7 +330,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     } else {
         const uint32_t quarter = warp & 3u, row = quarter * 32u + lane, t = t_first + row;
         const uint32_t lane_base = tmem + ((quarter * 32u) << 16);
-        const float mul = rsqrtf((float)D) * kLog2e;
+        const float mul = rsqrtf((float)D) * kLog2e / (kWindowHeld * kWindowHeld);
         // what column t sees: [lo, t] and [s0, s0 + sk)
         const uint32_t s0 = t / a.seq_len * a.seq_len;
         const uint32_t lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0;

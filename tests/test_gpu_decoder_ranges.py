@@ -110,3 +110,28 @@ def test_scores_of_some_tens(dim, window, size):
     want, bound = D.window_attention(x[:rq], x[rq: rq + rk], x[rq + rk:], h_q, h_kv, seq, columns, window, 3, ops.THETA)
     ops.within(ops.read(canvas, pitch)[rq + 2 * rk:, :columns], want, bound, "window attention")
     plan.close()
+
+
+# ---- rotations that leave FP16 --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("loud", ["queries", "keys"])
+def test_window_attention_with_rotations_beyond_fp16(dim, loud):
+    """A pair of 6e4 and 6e4 is as long as 84852, which is no FP16 number; the scores are ordinary."""
+    seq, columns = 150, 290
+    rng = np.random.default_rng(dim)
+    pitch = ops.pitch_of(columns)
+    body = rng.normal(0, 1, (3 * dim, pitch)).astype(np.float16)
+    big, small = (0, dim) if loud == "queries" else (dim, 0)
+    body[big: big + dim] = 0
+    for p in (0, 5, dim // 2 - 1):
+        body[big + p], body[big + p + dim // 2] = 60000, rng.choice([-60000, 60000], pitch)
+    body[small: small + dim] *= np.float16(2.0 ** -10)
+    plan, canvas = ops.make_plan(body, dim, columns)
+    plan.add_window_attn(0, dim * pitch, 2 * dim * pitch, 3 * dim * pitch, 1, 1, dim, seq, theta=ops.THETA)
+    plan.execute()
+    assert plan.status() == 0
+    x = body[:, :columns].astype(np.float64)
+    want, bound = D.window_attention(x[:dim], x[dim: 2 * dim], x[2 * dim:], 1, 1, seq, columns, 0, 0, ops.THETA)
+    assert np.isfinite(want).all() and np.median(bound) < 0.2, "the bound says something"
+    ops.within(ops.read(canvas, pitch)[3 * dim:, :columns], want, bound, "window attention")
+    plan.close()
