@@ -260,8 +260,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
 // rounded to FP16 is a weight relative to the largest one, not to that times its block's scale, or one loud block (a value of
 // 6e4 next to values of 1) would leave nothing of the weights behind it. p' <= 1 is held as 2^15 p', so that FP16 has whole
 // precision down to 2^-29 and something down to 2^-40 of the largest weight.
-// q is split into two FP16 numbers (high and low part): with exact codes the scores are then as good as in 32 bits. With up to 8
-// heads the low parts are rows 8 to 15 of the operand, which would be empty, and cost nothing.
+// Half of q (a rotated pair of FP16 numbers may be sqrt(2) longer than the largest one) is split into two FP16 numbers (high and low
+// part): with exact codes the scores are then as good as in 32 bits. With up to 8 heads the low parts are rows 8 to 15 of the operand,
+// which would be empty, and cost nothing.
 // Measured, both launches: 48 columns at up to 8190 positions, 32 heads on 8 of 128 dimensions: 78 to 80 us for 348 MB (4.4 TB/s; the
 // same without the products: what bounds it is bytes in flight and the last warps' end); 64 columns at 511, D = 64, each
 // completing a block: 24 us; 64 columns at up to 16000 with a window of 1024: 28; one column at 1500: 15, a chain of latencies.
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs 
                             const int i = 4 * s + 2 * t + e;
                             float u = __half2float(lo16[i]), v = __half2float(lo16[i + D / 2]);
                             rotate(u, v, __ldg(cs + p0 + i));
-                            y[e] = d0 < D / 2 ? u : v;
+                            y[e] = 0.5f * (d0 < D / 2 ? u : v);
                         }
                         hi[t] = pack2(y[0], y[1]);
                         const float2 hf = half2_of(hi[t]);
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
     }
     if (at.unit >= at.seen.units) next_head(at);                            // the share begins inside an open block's weight
     // ---- q of a (column, head) as operands, and the scales of 32 of its blocks: a lane holds those of one ----
-    const float sm = rsqrtf((float)D) * kLog2e;
+    const float sm = 2.0f * rsqrtf((float)D) * kLog2e;                      // of halves of q
     uint32_t qh[R][KS][2], ql[R][KS][2];
     float sc_mul = 0.f, sc_log = 0.f, sc_inv = 0.f;
     int sc_exp = 0;

@@ -135,3 +135,21 @@ def test_window_attention_with_rotations_beyond_fp16(dim, loud):
     assert np.isfinite(want).all() and np.median(bound) < 0.2, "the bound says something"
     ops.within(ops.read(canvas, pitch)[3 * dim:, :columns], want, bound, "window attention")
     plan.close()
+
+
+@pytest.mark.parametrize("h_q,dim", [(4, 64), (12, 64), (2, 128), (16, 128)])
+def test_kv8_attention_with_queries_beyond_fp16(h_q, dim):
+    """As above for the queries of single tokens."""
+    positions = np.array([1, 5, 63, 64, 130, 200], dtype=np.int32)
+    d = ops.Decoder(h_q, 1, dim, positions.size, 256, seed=dim)
+    d.history()
+    v = d.cache.views()
+    v["scales"][..., 0] *= 2.0 ** -12
+    v["k_tail"].mul_(2.0 ** -10)
+    body = d.rng.normal(0, 1, (d.rq + 2 * dim, d.pitch)).astype(np.float16)
+    body[: d.rq] = 0
+    for h in range(h_q):
+        body[h * dim + 3], body[h * dim + 3 + dim // 2] = 60000, d.rng.choice([-60000, 60000], d.pitch)
+    body[d.rq: d.rq + dim] *= np.float16(2.0 ** -10)
+    d.step(positions, body=body)
+    d.plan.close()
