@@ -167,7 +167,8 @@ int k44b_plan_add_window_attn(void *plan, const char *name, uint64_t q_off, uint
  *   scales     [column][head][block][keys, values] FP32
  *   k_tail     [column][head][64 positions][head_dim] FP16       v_tail  [column][head][head_dim][64 positions] FP16
  *   tail_block [column][head] int32, number of the open block, -1 none
- * Infinities count as +-65504; a NaN stays a NaN of its own value. k44b_kv8_bytes returns 0 for impossible sizes. */
+ * Keys are held rotated, rounded to FP16; finite ones beyond +-65504 (a rotated pair may be sqrt(2) longer) are held as that. In 8 bits
+ * infinities count as +-65504; a NaN stays a NaN of its own value. k44b_kv8_bytes returns 0 for impossible sizes. */
 typedef struct k44b_kv8_cache {
     void *data;
     uint64_t bytes;

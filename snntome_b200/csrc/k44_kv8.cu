@@ -2,7 +2,7 @@
 //
 // Format (k44_decoder.cuh): blocks of 64 tokens of one column and head, e4m3 codes with one FP32 scale per block for keys and
 // one for values,  scale = max(amax, 2^-24) / 448,  code = e4m3(x / scale);  infinities count as the largest FP16 number, a NaN
-// stays a NaN of its own value. The open block is kept as FP16 rows, so that a scale is chosen once, with all 64 tokens known.
+// stays a NaN of its own value; keys are rotated, and rounded to FP16, where finite ones end at the largest number. The open block is kept as FP16 rows, so that a scale is chosen once, with all 64 tokens known.
 // A block is brought to 8 bits by the step that appends its last token and read in 8 bits from the next block on.
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
@@ -39,6 +39,10 @@ __device__ __forceinline__ void rotate(float &a, float &b, float2 cs) {
     a = x;
 }
 
+// A rotated pair of FP16 numbers may be sqrt(2) longer than the largest one; in the cache such a key is the largest number. Infinities
+// and NaN stay what they are.
+__device__ __forceinline__ float held(float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x; }
+
 // ---- 8 bits -------------------------------------------------------------------------------------------------------------------
 // largest magnitudes so far, two at a time; the maximum of a number and a NaN is the number
 __device__ __forceinline__ __half2 amax_of(__half2 m, uint32_t two) { return __hmax2(m, __habs2(*reinterpret_cast<const __half2 *>(&two))); }
@@ -61,6 +65,12 @@ __device__ __forceinline__ float2 half2_of(uint32_t u) { return __half22float2(*
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+// the same, and what is beyond the largest number becomes that; a NaN stays one
+__device__ __forceinline__ uint32_t pack2_finite(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
 }
 
 // ---- filling the cache from a prompt ----------------------------------------------------------------------------------------
@@ -149,10 +159,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
             if (h != h0) __syncthreads();
             stage_all();
             if (h + 1u < h1) fetch(h + 1u);
-            __half2 amax = __float2half2_rn(0.f);
-            uint32_t lo[ROUNDS][4], hi[ROUNDS][4];
-#pragma unroll
-            for (uint32_t r = 0; r < ROUNDS; ++r) {
+            // a round's token: its 8 pairs, rotated and rounded by `pack`
+            auto turn = [&](uint32_t r, uint32_t (&lo)[4], uint32_t (&hi)[4], auto pack) {
                 const __half *x = xs + p0 * ROW + shift + r * TOKENS + tok0;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
@@ -163,12 +171,19 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
                         v[e] = __half2float(x[(2 * i + e + D / 2) * ROW]);
                         rotate(u[e], v[e], cs[r][2 * i + e]);
                     }
-                    lo[r][i] = pack2(u[0], u[1]);
-                    hi[r][i] = pack2(v[0], v[1]);
-                    amax = amax_of(amax_of(amax, lo[r][i]), hi[r][i]);
+                    lo[i] = pack(u[0], u[1]);
+                    hi[i] = pack(v[0], v[1]);
                 }
-            }
-            if (n == kKv8Block) {                                    // a whole block: 8 bits
+            };
+            if (n == kKv8Block) {                                    // a whole block: 8 bits, where infinities too count as the largest number
+                __half2 amax = __float2half2_rn(0.f);
+                uint32_t lo[ROUNDS][4], hi[ROUNDS][4];
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; ++r) {
+                    turn(r, lo[r], hi[r], [](float x, float y) { return pack2_finite(x, y); });
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) amax = amax_of(amax_of(amax, lo[r][i]), hi[r][i]);
+                }
                 const float scale = scale_of(whole_max(amax_of(amax))), inv = 1.0f / scale;
                 uint8_t *codes = a.cache.codes + (ch * a.cache.blocks + block) * (2u * kKv8Block * D);
                 if (tid == 0u) a.cache.scales[ch * a.cache.blocks + block].x = scale;
@@ -185,8 +200,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
                 for (uint32_t r = 0; r < ROUNDS; ++r) {
                     const uint32_t t = r * TOKENS + tok0;
                     if (t >= n) continue;
-                    *reinterpret_cast<uint4 *>(tail + t * D + p0) = make_uint4(lo[r][0], lo[r][1], lo[r][2], lo[r][3]);
-                    *reinterpret_cast<uint4 *>(tail + t * D + p0 + D / 2) = make_uint4(hi[r][0], hi[r][1], hi[r][2], hi[r][3]);
+                    uint32_t lo[4], hi[4];
+                    turn(r, lo, hi, [](float x, float y) { return pack2(held(x), held(y)); });
+                    *reinterpret_cast<uint4 *>(tail + t * D + p0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    *reinterpret_cast<uint4 *>(tail + t * D + p0 + D / 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 }
             }
         }
@@ -405,7 +422,7 @@ __global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs 
         if (is_k) {
             float u = __half2float(x[p]), v = __half2float(x[p + D / 2]);
             rotate(u, v, __ldg(cs + p));
-            const __half hu = __float2half_rn(u), hv = __float2half_rn(v);
+            const __half hu = __float2half_rn(held(u)), hv = __float2half_rn(held(v));
             tail[slot * D + p] = hu; tail[slot * D + p + D / 2] = hv;
             x[p] = hu; x[p + D / 2] = hv;
         } else {

@@ -153,3 +153,43 @@ def test_kv8_attention_with_queries_beyond_fp16(h_q, dim):
     body[d.rq: d.rq + dim] *= np.float16(2.0 ** -10)
     d.step(positions, body=body)
     d.plan.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cached_keys_beyond_fp16_are_held_as_the_largest_number(dim):
+    """Finite keys stay finite, from a prompt and token by token; an infinity stays one in the open block."""
+    import torch
+    n, h_kv = 70, 2
+    rk, pitch = h_kv * dim, 128
+    rng = np.random.default_rng(dim)
+    body = rng.normal(0, 1, (2 * rk, pitch)).astype(np.float16)
+    body[4, :], body[4 + dim // 2, :] = 60000, rng.choice([-60000, 60000], pitch)
+    body[rk - 1, 66] = np.inf
+    cache = ops.KV8Cache(1, h_kv, dim, 128)
+    plan, _ = ops.make_plan(body, 0, n)
+    plan.add_kv8_fill(cache, 0, rk * pitch, n, theta=ops.THETA)
+    plan.set_sequences([0], [n])
+    plan.execute()
+    assert plan.status() == 0
+    plan.close()
+    a = ops.cache_arrays(cache)
+    k = D.rotated(body[:dim, :n].astype(np.float64).T, np.arange(n), ops.THETA)
+    assert np.abs(k).max() > 80000
+    held = np.clip(k, -65504, 65504)
+    row = a["k_tail"][0, 0, :6].astype(np.float64)
+    assert np.all(np.abs(row - held[64:]) <= D.HALF16 * np.abs(held[64:]) + 2.0 ** -22 * np.abs(k).max() + D.TINY16)
+    assert np.isinf(a["k_tail"][0, 1, 2, dim - 1]), "an infinity"
+    got = ops.block_values(a, 0, 0, 0, dim)[0]
+    assert abs(a["scales"][0, 0, 0, 0] / (65504 / 448) - 1) <= 2.0 ** -23
+    scale = 65504 / 448
+    assert np.all(np.abs(got - held[:64]) <= (D.e4m3_half_step(np.abs(held[:64]) / scale * (1 + 2 * D.HALF16)) * scale + D.HALF16 * np.abs(held[:64]) * 1.01 + 2.0 ** -22 * np.abs(k).max()) * 1.001)
+    # the same tokens one by one
+    one = ops.Decoder(h_kv, h_kv, dim, 1, 128)
+    for t in range(n):
+        x = np.zeros((3 * rk, one.pitch), dtype=np.float16)
+        x[rk:, 0] = body[:, t]
+        one.step([t], tag=False, check=False, body=x)
+    for part, b in ops.cache_arrays(one.cache).items():
+        if part != "tail_block":
+            assert np.array_equal(b[..., :6, :] if part == "k_tail" else b[..., :6] if part == "v_tail" else b[:, :, :1], a[part][..., :6, :] if part == "k_tail" else a[part][..., :6] if part == "v_tail" else a[part][:, :, :1], equal_nan=part != "codes"), part
+    one.plan.close()
