@@ -199,6 +199,12 @@ bool Executor::check(cudaError_t e, const char *what) {
     return false;
 }
 
+// Clears on the default stream, and waits for that: what comes next to this memory may come on a stream that does not.
+static cudaError_t clear_now(void *p, int fill, size_t bytes) {
+    const cudaError_t e = cudaMemsetAsync(p, fill, bytes, cudaStreamLegacy);
+    return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
+}
+
 void Executor::release() {
     if (device_ >= 0) cudaSetDevice(device_);
     for (auto &w : waves_) {
@@ -264,9 +270,9 @@ bool Executor::begin(int device, uint64_t canvas_elems, uint32_t pitch, uint32_t
     if (canvas_elems == 0 || canvas_elems % 8u) return fail("canvas size must be a positive multiple of 8 elements");
     pitch_ = pitch; columns_ = columns ? columns : pitch; canvas_elems_ = canvas_elems;
     if (!check(cudaMalloc(&canvas_, canvas_elems * sizeof(__half)), "canvas allocation")) { canvas_ = nullptr; return false; }
-    if (!check(cudaMemset(canvas_, 0, canvas_elems * sizeof(__half)), "canvas clear")) return false;
+    if (!check(clear_now(canvas_, 0, canvas_elems * sizeof(__half)), "canvas clear")) return false;
     if (!check(cudaMalloc(&d_status_, kStatusBytes), "status allocation")) return false;
-    if (!check(cudaMemset(d_status_, 0, kStatusBytes), "status clear")) return false;
+    if (!check(clear_now(d_status_, 0, kStatusBytes), "status clear")) return false;
     if (!check(cudaEventCreate(&ev0_), "event") || !check(cudaEventCreate(&ev1_), "event")) return false;
     if (!check(umma_kernel_setup(), "kernel attribute setup") || !check(mma_kernel_setup(), "kernel attribute setup")) return false;
     return true;
@@ -324,15 +330,15 @@ int *Executor::decode_pos_ptr() {
     if (!ready()) { fail("executor not initialised"); return nullptr; }
     if (!d_pos_) {
         if (!check(cudaSetDevice(device_), "cudaSetDevice") || !check(cudaMalloc(&d_pos_, sizeof(int)), "position word allocation") ||
-            !check(cudaMemset(d_pos_, 0, sizeof(int)), "position word clear"))
+            !check(clear_now(d_pos_, 0, sizeof(int)), "position word clear"))
             return nullptr;
     }
     return d_pos_;
 }
 
-static int *alloc_words(int device, uint32_t n, std::string &err) {
+static int *alloc_words(int device, uint32_t n, std::string &err, int fill = 0) {
     int *p = nullptr;
-    if (cudaSetDevice(device) != cudaSuccess || cudaMalloc(&p, (size_t)n * sizeof(int)) != cudaSuccess || cudaMemset(p, 0, (size_t)n * sizeof(int)) != cudaSuccess) {
+    if (cudaSetDevice(device) != cudaSuccess || cudaMalloc(&p, (size_t)n * sizeof(int)) != cudaSuccess || clear_now(p, fill, (size_t)n * sizeof(int)) != cudaSuccess) {
         err = "token buffer allocation failed";
         cudaFree(p);
         return nullptr;
@@ -485,8 +491,7 @@ bool Executor::add_aux(const HostWave &w) {
 int *Executor::positions_ptr() {
     if (!ready()) { fail("executor not initialised"); return nullptr; }
     if (!d_positions_) {
-        if (!(d_positions_ = alloc_words(device_, pitch_, err))) return nullptr;
-        if (!check(cudaMemset(d_positions_, 0xff, (size_t)pitch_ * sizeof(int)), "positions clear")) return nullptr;      // -1: idle
+        if (!(d_positions_ = alloc_words(device_, pitch_, err, 0xff))) return nullptr;                                    // -1: idle
         for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_ARGMAX && o.aux.advance) o.aux.positions = d_positions_;
         drop_graph();                               // a graph captured before holds the old arguments
     }
@@ -496,10 +501,9 @@ int *Executor::positions_ptr() {
 int2 *Executor::sequences_ptr() {
     if (!ready()) { fail("executor not initialised"); return nullptr; }
     if (!d_sequences_) {
-        int *p = alloc_words(device_, 2u * pitch_, err);
+        int *p = alloc_words(device_, 2u * pitch_, err, 0xff);                                                             // column -1: skip
         if (!p) return nullptr;
         d_sequences_ = (int2 *)p;
-        if (!check(cudaMemset(p, 0xff, (size_t)pitch_ * sizeof(int2)), "sequence table clear")) return nullptr;            // column -1: skip
     }
     return d_sequences_;
 }
@@ -567,7 +571,7 @@ bool Executor::reserve(void *&p, uint64_t &have, uint64_t need, const char *what
     if (need <= have) return true;
     void *grown = nullptr;
     if (!check(cudaDeviceSynchronize(), "synchronise") || !check(cudaMalloc(&grown, need), what)) return false;
-    if (!check(cudaMemset(grown, 0, need), what) || !check(cudaDeviceSynchronize(), what)) { cudaFree(grown); return false; }
+    if (!check(clear_now(grown, 0, need), what)) { cudaFree(grown); return false; }
     drop_graph();                                   // one captured before holds the old buffer
     cudaFree(p);
     p = grown; have = need;
@@ -1090,7 +1094,7 @@ bool Executor::reserve_scratch(size_t tiles) {
     const size_t sb = tiles * 64u * kTileM * sizeof(float), cb = tiles * sizeof(uint32_t);
     if (!check(cudaMalloc(&d_scratch_, sb), "split-K scratch allocation") || !check(cudaMalloc(&d_counters_, cb), "split-K counter allocation"))
         return false;
-    if (!check(cudaMemset(d_scratch_, 0, sb), "scratch clear") || !check(cudaMemset(d_counters_, 0, cb), "counter clear")) return false;
+    if (!check(clear_now(d_scratch_, 0, sb), "scratch clear") || !check(clear_now(d_counters_, 0, cb), "counter clear")) return false;
     scratch_tiles_ = tiles;
     drop_graph();
     return true;

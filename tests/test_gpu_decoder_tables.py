@@ -1,0 +1,87 @@
+"""The tables that the decoder operators read (positions, sequences), their scratch under captured graphs, and positions at the ends of a
+cache and of its blocks."""
+import numpy as np
+import pytest
+
+import test_gpu_decoder_ops as ops
+from oracle import decoder as D
+from snntome_b200.native import KV8Cache, NativeError, NativePlan
+
+pytestmark = pytest.mark.gpu
+
+
+def busy_default_stream():
+    """Some tens of milliseconds of work on the default stream, and a stream that does not wait for it."""
+    import torch
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    torch.cuda._sleep(100_000_000)
+    return s
+
+
+def test_positions_set_before_the_command_on_a_stream_of_their_own():
+    import torch
+    h_q, h_kv, dim = 2, 1, 64
+    pitch = 64
+    rng = np.random.default_rng(1)
+    body = rng.normal(0, 1, (4 * dim, pitch)).astype(np.float16)
+    out = []
+    for early in (False, True):
+        plan, canvas = ops.make_plan(body, 2 * dim, 3)
+        cache = KV8Cache(3, h_kv, dim, 100)
+        torch.cuda.synchronize()
+        s = torch.cuda.current_stream()
+        if early:
+            s = busy_default_stream()
+            plan.set_positions([0, -1, 0], stream=s)
+        plan.add_kv8_attn(cache, 0, 2 * dim * pitch, 3 * dim * pitch, 4 * dim * pitch, h_q)
+        if not early:
+            plan.set_positions([0, -1, 0])
+        plan.execute(stream=s)
+        assert plan.status() == 0
+        out.append(ops.read(canvas, pitch)[4 * dim:, :3].copy())
+        plan.close()
+    assert out[0][:, 0].any() and np.array_equal(out[0].view(np.uint16), out[1].view(np.uint16))
+
+
+@pytest.mark.parametrize("first", ["table", "command"])
+def test_sequences_set_on_a_stream_of_their_own(first):
+    import torch
+    h_kv, dim, seq = 2, 64, 70
+    rk, pitch = h_kv * dim, 256
+    body = np.random.default_rng(2).normal(0, 1, (2 * rk, pitch)).astype(np.float16)
+    plan, canvas = ops.make_plan(body, rk, 3 * seq)
+    plan.add_window_attn(0, 0, rk * pitch, 2 * rk * pitch, h_kv, h_kv, dim, seq)          # its angles are those of the filling too
+    cache = KV8Cache(4, h_kv, dim, 100)
+    if first == "table":
+        s = busy_default_stream()
+        plan.set_sequences([3, -1, 0], [70, 70, 64], stream=s)
+        plan.add_kv8_fill(cache, 0, rk * pitch, seq)
+    else:
+        s = busy_default_stream()
+        plan.add_kv8_fill(cache, 0, rk * pitch, seq)
+        plan.set_sequences([3, -1, 0], [70, 70, 64], stream=s)
+    plan.execute(stream=s)
+    assert plan.status() == 0
+    a = ops.cache_arrays(cache)
+    assert a["tail_block"].tolist() == [[-1, -1], [-1, -1], [-1, -1], [1, 1]] and (a["scales"][[0, 3], :, 0] > 0).all()
+    plan.close()
+
+
+def test_a_plan_made_and_used_while_the_default_stream_is_busy():
+    """Its canvas is clear when the call returns, so that what other streams write then stays."""
+    import torch
+    body = torch.randn(8 * 64, 64, device="cuda").to(torch.float16)
+    out = []
+    for busy in (False, True):
+        s = busy_default_stream() if busy else torch.cuda.Stream()
+        plan = NativePlan.create(14 * 64 * 64, 64, 50)
+        with torch.cuda.stream(s):
+            canvas = plan.canvas_tensor()
+            canvas[: body.numel()].copy_(body.reshape(-1))
+            plan.add_window_attn(0, 2 * 64 * 64, 3 * 64 * 64, 8 * 64 * 64, 2, 1, 64, 50)
+            plan.execute(stream=s)
+        assert plan.status() == 0
+        out.append(canvas.clone())
+        plan.close()
+    assert bool(out[0][8 * 64 * 64:].any()) and torch.equal(out[0], out[1])
