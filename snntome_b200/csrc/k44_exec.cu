@@ -215,6 +215,8 @@ void Executor::release() {
     cudaFree(d_scratch_); d_scratch_ = nullptr;
     cudaFree(d_counters_); d_counters_ = nullptr;
     scratch_tiles_ = 0;
+    for (void *p : retired_) cudaFree(p);
+    retired_.clear();
     for (void *p : ipc_opened_) cudaIpcCloseMemHandle(p);
     ipc_opened_.clear();
     cudaFree(d_pos_); d_pos_ = nullptr;
@@ -405,7 +407,7 @@ bool Executor::add_aux(const HostWave &w) {
             const size_t pbytes = (size_t)((w.max_seq + kDecodeChunk - 1u) / kDecodeChunk) * w.h_q * kDecodeRow * pitch_ * sizeof(float);
             if (pbytes > decode_partial_bytes_) {
                 if (!check(cudaDeviceSynchronize(), "synchronise")) return false;
-                cudaFree(d_decode_partial_); d_decode_partial_ = nullptr; decode_partial_bytes_ = 0;
+                retire(d_decode_partial_); d_decode_partial_ = nullptr; decode_partial_bytes_ = 0;
                 if (!check(cudaMalloc(&d_decode_partial_, pbytes), "attention scratch allocation")) return false;
                 decode_partial_bytes_ = pbytes;
                 for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_DECODE_ATTN) o.aux.partial = d_decode_partial_;
@@ -434,7 +436,7 @@ bool Executor::add_aux(const HostWave &w) {
         const size_t words = (size_t)((w.cout + kArgmaxChunk - 1u) / kArgmaxChunk) * pitch_;
         if (words > argmax_words_) {
             if (!check(cudaDeviceSynchronize(), "synchronise")) return false;
-            cudaFree(d_argmax_); d_argmax_ = nullptr; argmax_words_ = 0;
+            retire(d_argmax_); d_argmax_ = nullptr; argmax_words_ = 0;
             if (!check(cudaMalloc(&d_argmax_, words * sizeof(unsigned long long)), "arg-max scratch allocation")) return false;
             argmax_words_ = words;
             for (auto &o : waves_) if (o.is_aux && o.aux.kind == AUX_ARGMAX) o.aux.argmax_scratch = d_argmax_;
@@ -573,7 +575,7 @@ bool Executor::reserve(void *&p, uint64_t &have, uint64_t need, const char *what
     if (!check(cudaDeviceSynchronize(), "synchronise") || !check(cudaMalloc(&grown, need), what)) return false;
     if (!check(clear_now(grown, 0, need), what)) { cudaFree(grown); return false; }
     drop_graph();                                   // one captured before holds the old buffer
-    cudaFree(p);
+    retire(p);
     p = grown; have = need;
     return true;
 }
@@ -1089,7 +1091,7 @@ bool Executor::init(const HostPlan &plan, int device, int force_path) {
 bool Executor::reserve_scratch(size_t tiles) {
     if (tiles <= scratch_tiles_) return true;
     if (!check(cudaDeviceSynchronize(), "synchronise")) return false;
-    cudaFree(d_scratch_); cudaFree(d_counters_);
+    retire(d_scratch_); retire(d_counters_);
     d_scratch_ = nullptr; d_counters_ = nullptr; scratch_tiles_ = 0;
     const size_t sb = tiles * 64u * kTileM * sizeof(float), cb = tiles * sizeof(uint32_t);
     if (!check(cudaMalloc(&d_scratch_, sb), "split-K scratch allocation") || !check(cudaMalloc(&d_counters_, cb), "split-K counter allocation"))
@@ -1098,6 +1100,11 @@ bool Executor::reserve_scratch(size_t tiles) {
     scratch_tiles_ = tiles;
     drop_graph();
     return true;
+}
+
+// Scratch that a larger one has replaced. A graph that the caller captured may still hold it, so it lives as long as the plan.
+void Executor::retire(void *p) {
+    if (p) retired_.push_back(p);
 }
 
 void Executor::drop_graph() {

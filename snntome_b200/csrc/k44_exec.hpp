@@ -143,6 +143,7 @@ class Executor {
     void recover_after_abort();
     bool launch_one(DeviceWave &w, cudaStream_t stream, uint32_t peer_slack = 0);
     void drop_graph();
+    void retire(void *p);
     void build_groups();
     bool launch_group(size_t gi, cudaStream_t stream);
     struct LaunchGroup { std::vector<size_t> waves; WaveGroupArgs args; uint32_t peer_slack = 0; };
@@ -173,6 +174,7 @@ class Executor {
     size_t argmax_words_ = 0;
     float *d_decode_partial_ = nullptr;   // per-chunk partial attention results, shared by all decode-attention commands
     size_t decode_partial_bytes_ = 0;
+    std::vector<void *> retired_;         // outgrown scratch, which captured graphs may hold
     // decoder operators: tables and scratch shared by all commands of the plan (they run one after the other)
     struct RopeTable { float theta; bool llama3, pairs_first; uint32_t head_dim, positions; float2 *d; };
     std::vector<RopeTable> rope_tables_;

@@ -85,3 +85,55 @@ def test_a_plan_made_and_used_while_the_default_stream_is_busy():
         out.append(canvas.clone())
         plan.close()
     assert bool(out[0][8 * 64 * 64:].any()) and torch.equal(out[0], out[1])
+
+
+def test_a_captured_graph_keeps_its_scratch_when_commands_are_added():
+    """Captured by the caller, then larger commands of every kind; what the graph holds must not be given to others meanwhile."""
+    import torch
+    h_q, h_kv, dim, pitch, columns, rows = 4, 2, 64, 64, 40, 1000
+    rq, rk = h_q * dim, h_kv * dim
+    rng = np.random.default_rng(3)
+    body = rng.normal(0, 1, (rq + 2 * rk + rows, pitch)).astype(np.float16)
+    plan, canvas = ops.make_plan(body, 2 * rq + 8192, columns)
+    out, late = (rq + 2 * rk + rows) * pitch, (2 * rq + rq + 2 * rk + rows) * pitch
+    cache = KV8Cache(columns, h_kv, dim, 400)
+    cache.storage[: cache.storage.numel() // 2] = 20
+    cache.views()["scales"].fill_(0.01)
+    cache.views()["tail_block"].fill_(4)
+    plan.add_window_attn(0, rq * pitch, (rq + rk) * pitch, out, h_q, h_kv, dim, 20, window=5)
+    plan.add_kv8_attn(cache, 0, rq * pitch, (rq + rk) * pitch, out + rq * pitch, h_q)
+    f = lambda *s: torch.zeros(s, device="cuda")
+    ent, rows_t, lp_t = f(columns), torch.zeros(3, columns, dtype=torch.int32, device="cuda"), f(3, columns)
+    plan.add_logprobs((rq + 2 * rk) * pitch, rows, entropy=ent, top_rows=rows_t, top_logprobs=lp_t)
+    plan.add_argmax((rq + 2 * rk) * pitch, rows)
+    plan.set_positions(np.full(columns, 300))
+    plan.execute()
+    assert plan.status() == 0
+    want = [canvas[out: late].clone(), ent.clone(), rows_t.clone(), lp_t.clone(), plan.next_tokens(columns)]
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+        plan.execute(stream=s)
+    # larger ones: more heads, wider groups, more rows
+    plan.add_window_attn(0, 0, 0, late, 4, 4, 64, 20)
+    for heads, kv, d in ((5, 1, 128), (9, 1, 128), (4, 4, 64)):
+        plan.add_kv8_attn(KV8Cache(columns, kv, d, 400), 0, 0, 0, late, heads)
+    plan.add_logprobs(0, 6000, entropy=f(columns))
+    plan.add_argmax(0, 6000)
+    torch.cuda.synchronize()
+    taken = [torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda") for n in (1 << 12, 1 << 14, 1 << 16, 1 << 18, 1 << 20, 1 << 21, 1 << 22) for _ in range(4)]
+    canvas[out: late] = float(ops.SENTINEL)
+    for t in (ent, rows_t, lp_t):
+        t.zero_()
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert plan.status() == 0
+    got = [canvas[out: late], ent, rows_t, lp_t, plan.next_tokens(columns)]
+    for a, b in zip(got[:4], want[:4]):
+        assert torch.equal(a, b)
+    assert np.array_equal(got[4], want[4])
+    for t in taken:
+        assert bool((t == 0x7f).all()), "the graph wrote into memory that is someone else's"
+    del g
+    plan.close()
