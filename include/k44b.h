@@ -178,8 +178,8 @@ uint64_t k44b_kv8_bytes(uint32_t columns, uint32_t h_kv, uint32_t head_dim, uint
 int k44b_kv8_clear(const k44b_kv8_cache *cache, void *stream);
 /* Prompt into the cache: the keys (not yet rotated; they are rotated at positions 0, 1, ... of their sequence) and values of a prompt
  * plan. set_sequences says, for the first n blocks of seq_len columns, which cache column a sequence goes to (-1: nowhere; no column
- * twice) and how long it is; blocks from n on go nowhere. What the column held before is replaced; positions from the length on are
- * left as they were. */
+ * twice) and how long it is (0: the column is empty then); blocks from n on go nowhere, and one that starts behind the plan's last
+ * column may not go anywhere either. What the column held before is replaced; positions from the length on are left as they were. */
 int k44b_plan_add_kv8_fill(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t k_off, uint64_t v_off, uint32_t seq_len, float rope_theta,
                            int llama3_scaling);
 int k44b_plan_set_sequences(void *plan, const int32_t *h_cache_columns, const int32_t *h_lengths, uint32_t n, void *stream);

@@ -531,7 +531,8 @@ static bool sequences_fit(const Kv8FillArgs &f, const std::vector<int32_t> &slot
         if (slots[i] < 0) continue;
         if ((uint32_t)slots[i] >= f.cache.columns) { why = "cache column " + std::to_string(slots[i]) + " does not exist"; return false; }
         if ((uint32_t)lengths[i] > f.seq_len || (uint32_t)lengths[i] > f.cache.max_seq) { why = "length " + std::to_string(lengths[i]) + " exceeds the sequence or the cache"; return false; }
-        if ((uint64_t)i * f.seq_len + (uint32_t)lengths[i] > f.columns) { why = "sequence " + std::to_string(i) + " leaves the plan's columns"; return false; }
+        // one of no tokens too starts inside the plan: blocks of columns that do not exist are not launched, and would not empty its cache column
+        if ((uint64_t)i * f.seq_len + std::max(1u, (uint32_t)lengths[i]) > f.columns) { why = "sequence " + std::to_string(i) + " leaves the plan's columns"; return false; }
     }
     return true;
 }

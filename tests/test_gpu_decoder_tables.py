@@ -137,3 +137,28 @@ def test_a_captured_graph_keeps_its_scratch_when_commands_are_added():
         assert bool((t == 0x7f).all()), "the graph wrote into memory that is someone else's"
     del g
     plan.close()
+
+
+def test_a_sequence_behind_the_last_column_is_refused():
+    """One of no tokens too: its block of columns does not exist, so nothing would empty its cache column."""
+    plan = NativePlan.create(512 * 64, 64, 20)
+    cache = KV8Cache(4, 1, 64, 30)
+    cache.views()["tail_block"].fill_(0)
+    plan.add_kv8_fill(cache, 0, 64 * 64, 10)
+    with pytest.raises(NativeError):
+        plan.set_sequences([0, 1, 2], [10, 10, 0])
+    plan.set_sequences([0, 1, -1], [10, 0, 0])                       # a block that exists may be empty
+    plan.execute()
+    assert plan.status() == 0
+    assert cache.views()["tail_block"].flatten().tolist() == [0, -1, 0, 0]
+    plan.close()
+    plan = NativePlan.create(512 * 64, 64, 20)
+    plan.set_sequences([0, 1, 2], [10, 10, 0])
+    with pytest.raises(NativeError):
+        plan.add_kv8_fill(cache, 0, 64 * 64, 10)                    # the sequences set before do not fit it
+    plan.set_sequences([0, 1, 2], [9, 9, 0])
+    plan.add_kv8_fill(cache, 0, 64 * 64, 9)
+    plan.execute()
+    assert plan.status() == 0
+    assert cache.views()["tail_block"].flatten().tolist() == [0, 0, -1, 0]
+    plan.close()
