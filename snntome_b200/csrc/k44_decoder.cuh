@@ -114,7 +114,8 @@ void logprob_place(LogprobArgs &a, void *scratch, uint32_t num_sms);
 cudaError_t logprob_setup();
 cudaError_t launch_logprobs(const LogprobArgs &a, const CUtensorMap &map, bool pdl, cudaStream_t s);      // map: the logits as rows of `pitch`, boxes of 64 x 64
 
-// programmatic dependent launch, as in k44_valu.cu
+// programmatic dependent launch, as in k44_valu.cu. A grid may start while the one before it still writes: what that one leaves (canvas
+// rows, operands, parts) is read by ordinary loads (`__ldcg`) after the wait, and only what nobody writes while the grid exists by `__ldg`.
 __device__ __forceinline__ void dep_enter() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

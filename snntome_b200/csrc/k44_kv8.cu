@@ -113,9 +113,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
             const uint32_t e = 256u * i + tid, c = (e & 7u) * 8u;
-            next[i] = c < end ? __ldg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + (e >> 3)) * a.pitch + c)) : make_uint4(0, 0, 0, 0);
+            next[i] = c < end ? __ldcg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + (e >> 3)) * a.pitch + c)) : make_uint4(0, 0, 0, 0);
         }
-        if (end > 64u && tid < D) ninth = __ldg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + tid) * a.pitch + 64u));
+        if (end > 64u && tid < D) ninth = __ldcg(reinterpret_cast<const uint4 *>(rows + ((uint64_t)h * D + tid) * a.pitch + 64u));
     };
     auto stage = [&](uint32_t row, uint32_t c, uint4 x) {
         uint32_t *to = reinterpret_cast<uint32_t *>(xs + row * ROW + c);
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(256) k44_kv8_prepare_kernel(const Kv8AttnArgs 
     const uint32_t rows = is_q ? G * D : (uint32_t)D;
     const __half *rows_of = is_q ? a.q + (uint64_t)head * G * D * a.pitch : (is_k ? a.k : a.v) + (uint64_t)head * D * a.pitch;
     for (uint32_t r = tid; r < rows; r += 256u) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(rows_of + (uint64_t)r * a.pitch + c0));
+        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(rows_of + (uint64_t)r * a.pitch + c0));
         const __half *h = reinterpret_cast<const __half *>(&v);
 #pragma unroll
         for (int c = 0; c < 8; ++c) xs[c * PAD + r] = h[c];
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const uint4 w = __ldg(frag + (r * KS + k) * 32);
+                const uint4 w = __ldcg(frag + (r * KS + k) * 32);
                 qh[r][k][0] = w.x; qh[r][k][1] = w.y; ql[r][k][0] = w.z; ql[r][k][1] = w.w;
             }
         fetch_scales(at.unit);

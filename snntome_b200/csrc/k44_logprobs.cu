@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256) k44_logprob_parts_kernel(const LogprobArg
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             v[i] = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);         // rows past the end: probability 0
-            if (col0 < a.columns && group * kLogprobGroup + rl + RL * i < a.rows) v[i] = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)(RL * i) * a.pitch));
+            if (col0 < a.columns && group * kLogprobGroup + rl + RL * i < a.rows) v[i] = __ldcg(reinterpret_cast<const uint4 *>(src + (uint64_t)(RL * i) * a.pitch));
         }
         __half2 mx[4];
         add_group<CG>([&](int i) -> uint4 { return v[i]; }, mx, m, base, low, L, W);
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kFinalThreads) k44_logprob_final_kernel(const 
     const bool known = t >= 0 && (uint32_t)t < a.rows;
     if (known && tid == 0u) target = __half2float(a.x[(uint64_t)t * a.pitch + col]);
     for (uint32_t c = tid; c < a.chunks; c += kFinalThreads) {
-        const float4 p = __ldg(parts + c);
+        const float4 p = __ldcg(parts + c);
         join(M, L, W, p.x, p.y, p.z);
     }
     if (warp * 32u < a.chunks) {
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kFinalThreads) k44_logprob_final_kernel(const 
     // Four threads take every 64th group; the top-th largest of the 64 maxima is such a value (where there are as many), and hardly
     // more groups reach it than are needed. Their rows that reach it are listed and ranked by counting.
     const uint16_t *gm = a.group_max + (uint64_t)col * a.group_stride;
-    auto key_of = [&](uint32_t g) -> uint32_t { return g < a.groups ? ((uint32_t)__ldg(gm + g) << 16) | (65535u - g) : 0u; };
+    auto key_of = [&](uint32_t g) -> uint32_t { return g < a.groups ? ((uint32_t)__ldcg(gm + g) << 16) | (65535u - g) : 0u; };
     bool listed = false;
     if (a.top) {
         uint32_t mine = 0, key[8];                                      // the first 2048 groups stay in registers
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kFinalThreads) k44_logprob_final_kernel(const 
                 const uint32_t b = b0 + 32u * i + lane;
                 key[i] = 0u;
                 if (b < blocks) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(gm + 8u * b));
+                    const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(gm + 8u * b));
                     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                     uint32_t mx = 0;
 #pragma unroll
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kFinalThreads) k44_logprob_final_kernel(const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t place = 32u * i + lane, from = __shfl_sync(0xffffffffu, best, place >> 3), g = (65535u - (from & 0xffffu)) * 8u + (place & 7u);
-            key[i] = from && g < a.groups ? ((uint32_t)__ldg(gm + g) << 16) | (65535u - g) : 0u;
+            key[i] = from && g < a.groups ? ((uint32_t)__ldcg(gm + g) << 16) | (65535u - g) : 0u;
         }
         best = warp_top<8>(key, a.top, lane);
         // in the order of their rows, so that a place in the list orders rows too

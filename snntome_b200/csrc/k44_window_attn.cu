@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
         uint32_t bad = 0;
         for (uint32_t e = tid; e < D * 8u; e += 256u) {
             const uint32_t d = e >> 3, c = (e & 7u) * 8u;
-            uint4 x = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
+            uint4 x = __ldcg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
             uint32_t *w = reinterpret_cast<uint32_t *>(&x);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
     auto fetch = [&](uint32_t i) {
         const __half *src = a.k + (uint64_t)i * D * a.pitch + col0;
 #pragma unroll
-        for (int n = 0; n < D / 32; ++n) { const uint32_t e = 256u * n + tid; next[n] = __ldg(reinterpret_cast<const uint4 *>(src + (uint64_t)(e >> 3) * a.pitch + (e & 7u) * 8u)); }
+        for (int n = 0; n < D / 32; ++n) { const uint32_t e = 256u * n + tid; next[n] = __ldcg(reinterpret_cast<const uint4 *>(src + (uint64_t)(e >> 3) * a.pitch + (e & 7u) * 8u)); }
     };
     fetch(h0);
     for (h = h0; h < h1; ++h) {
