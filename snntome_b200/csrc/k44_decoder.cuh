@@ -81,9 +81,10 @@ struct WindowAttnArgs {
     const __half *q = nullptr, *k = nullptr, *v = nullptr;
     __half *out = nullptr;
     // re-laid operands: rotated k [h_kv][pitch][head_dim], v [h_kv * head_dim][pitch] with
-    // non-finite values replaced by zero, and per (head, 64 columns) whether there were any
+    // non-finite values replaced by zero, per (head, 64 columns) whether there were any, and which: [h_kv][64 columns][head_dim]
     __half *k_rows = nullptr, *v_rows = nullptr;
     uint32_t *v_flags = nullptr;
+    uint4 *v_marks = nullptr;
     const float2 *rope = nullptr, *rope_pairs = nullptr;       // [position][pair], [pair][position]: `positions` of them
     uint32_t *status = nullptr;
     uint32_t pitch = 0, columns = 0, h_q = 0, h_kv = 0, head_dim = 0, seq_len = 0, window = 0, sinks = 0, positions = 0;

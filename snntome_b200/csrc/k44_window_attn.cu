@@ -21,8 +21,10 @@ __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) !
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
 // CTA = 64 columns of a few heads of k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
-// not finite become zero too and are flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
-// tensor cores; the attention adds them to the columns that do see them. The rotated q and k, and the weights, are rounded to FP16, the
+// not finite become zero too, and their tile is flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
+// tensor cores; the attention adds them to the columns that do see them. A flagged tile leaves a word of 64 bits per dimension for the
+// columns that hold +inf (or NaN) and one for -inf (or NaN): a column of the output needs an AND with what it sees, not the values
+// (2048 columns, 8 heads on 2 of 64, one infinity for all to see: 47 us without, 1867 with the values read, 61 with the words). The rotated q and k, and the weights, are rounded to FP16, the
 // tensor cores' type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16. q and k are held at
 // half their size there: a pair of FP16 numbers may be sqrt(2) longer than the largest one, and halves are exact down to 2^-13.
 template <int D>
@@ -54,6 +56,28 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
         }
         const int any = __syncthreads_or((int)bad);
         if (tid == 0u) a.v_flags[h * (a.pitch / 64u) + tile] = any ? 1u : 0u;
+        if (!any) return;
+        uint4 *marks = a.v_marks + ((uint64_t)h * (a.pitch / 64u) + tile) * D;
+        for (uint32_t e = tid; e < D * 8u; e += 256u) {                      // eight neighbours hold a dimension
+            const uint32_t d = e >> 3, c = (e & 7u) * 8u;
+            const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(src + (uint64_t)d * a.pitch + c));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t up = 0, down = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                const uint32_t v = w[i >> 1] >> (16u * (i & 1u)) & 0xffffu;
+                if (finite_bits(v) || col0 + c + i >= a.columns) continue;
+                if (v != 0xfc00u) up |= 1u << i;
+                if (v != 0x7c00u) down |= 1u << i;
+            }
+            up <<= c & 31u; down <<= c & 31u;
+            uint32_t m[4] = {c < 32u ? up : 0u, c < 32u ? 0u : up, c < 32u ? down : 0u, c < 32u ? 0u : down};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) m[i] |= __shfl_xor_sync(0xffffffffu, m[i], o);
+            if ((e & 7u) == 0u) marks[d] = make_uint4(m[0], m[1], m[2], m[3]);
+        }
         return;
     }
     // A thread owns one token and 8 rotation pairs (16 bytes of either half of the token's row); neighbours own the next pairs, so that
@@ -162,6 +186,20 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
     return (0xffffffffu >> (31 - min(to, 31))) & (0xffffffffu << max(from, 0));
 }
 
+// what column t sees: [lo, t] and [s0, s0 + sk)
+struct Sight {
+    uint32_t t, s0, lo, sk;
+    __device__ __forceinline__ Sight(const WindowAttnArgs &a, uint32_t column) : t(column) {
+        s0 = t / a.seq_len * a.seq_len;
+        lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0;
+        sk = lo > s0 ? min(a.sinks, lo - s0) : 0u;
+    }
+    __device__ __forceinline__ uint32_t seen(uint32_t c0) const {           // of the 32 keys from c0
+        const int at = (int)c0;
+        return bits((int)lo - at, (int)t - at) | bits((int)s0 - at, (int)(s0 + sk) - 1 - at);
+    }
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, Shape<D>::CTAS)
 k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -174,7 +212,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const uint32_t q_full = ctl, k_full = ctl + 8u, k_empty = k_full + 8u * ST, v_full = k_empty + 8u * ST, v_empty = v_full + 8u * ST;
     const uint32_t s_full = v_empty + 8u * ST, p_full = s_full + 16u, pv_done = p_full + 16u;
     uint8_t *ctl_ptr = smem_raw + (ctl - ptx::smem_addr(smem_raw));
-    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(ctl_ptr + 192), *abort_word = tmem_slot + 1;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(ctl_ptr + 192), *abort_word = tmem_slot + 1, *flagged = tmem_slot + 2;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0) {
@@ -295,6 +333,10 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             }
         }
         __syncwarp();
+        bool any = false;                                                       // of this CTA's tiles with values that are not finite
+        for (uint32_t j = lane; j < n; j += 32u) any |= a.v_flags[hk * (a.pitch / 64u) + key_tile(j)] != 0u;
+        any = __any_sync(0xffffffffu, any) != 0;
+        if (lane == 0) *flagged = any ? 1u : 0u;
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc_s = (1u << 4) | ((kKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
@@ -331,14 +373,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         const uint32_t quarter = warp & 3u, row = quarter * 32u + lane, t = t_first + row;
         const uint32_t lane_base = tmem + ((quarter * 32u) << 16);
         const float mul = rsqrtf((float)D) * kLog2e / (kWindowHeld * kWindowHeld);
-        // what column t sees: [lo, t] and [s0, s0 + sk)
-        const uint32_t s0 = t / a.seq_len * a.seq_len;
-        const uint32_t lo = a.window && t - s0 >= a.window ? t - a.window + 1u : s0;
-        const uint32_t sk = lo > s0 ? min(a.sinks, lo - s0) : 0u;
-        auto seen = [&](uint32_t c0) -> uint32_t {                          // of the 32 keys from c0
-            const int at = (int)c0;
-            return bits((int)lo - at, (int)t - at) | bits((int)s0 - at, (int)(s0 + sk) - 1 - at);
-        };
+        const Sight sight(a, t);
         // Scores j are made after the product j - BUFFERS, so a warp that has seen them knows of the products up to j - 2 at least. A parity tells
         // two phases apart: with one barrier for all products, a warp ahead of the others would take the end of product j - 3 for
         // that of j - 1. So odd and even products have a barrier each.
@@ -354,7 +389,7 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             ptx::tc_fence_after();
             uint32_t r[32], r2[S::HOLD ? 32 : 1];                              // scores of the first 32 keys, and, where registers allow, of the others
             // Of 32 columns and 32 keys on an edge most see all or nothing: those need no mask, these no exponentials.
-            const uint32_t see0 = whole ? ~0u : seen(c0), see1 = whole ? ~0u : seen(c0 + 32u);
+            const uint32_t see0 = whole ? ~0u : sight.seen(c0), see1 = whole ? ~0u : sight.seen(c0 + 32u);
             const bool any0 = whole || __any_sync(0xffffffffu, see0 != 0u), any1 = whole || __any_sync(0xffffffffu, see1 != 0u);
             const bool all0 = whole || __all_sync(0xffffffffu, see0 == ~0u), all1 = whole || __all_sync(0xffffffffu, see1 == ~0u);
             auto hide = [&](uint32_t (&x)[32], uint32_t see) {
@@ -446,10 +481,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (ok) {
             ptx::tc_fence_after();
             const float inv = 1.0f / l;
-            // values that were kept from the tensor cores: a column that sees one gets it
-            bool flagged = false;
-            const uint32_t *flags = a.v_flags + hk * (a.pitch / 64u);
-            for (uint32_t j = 0; j < n; ++j) flagged |= flags[key_tile(j)] != 0u;
             // Rows of the output are columns of the canvas: 2 bytes per lane and dimension, 128 stores of 64 bytes each per warp, which took
             // 4500 cycles per item (D = 128). Whole tiles go through the shared memory that held q and out with tensor copies instead.
             __half *const out_s = reinterpret_cast<__half *>(smem_raw + (q_smem - ptx::smem_addr(smem_raw)));      // [half of the columns][dimension][64]
@@ -460,20 +491,6 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                 uint32_t o[32];
                 ptx::tmem_ld_32x32(lane_base + kOCol + d0, o);
                 ptx::tmem_ld_wait();
-                if (flagged && t < a.columns) {
-                    for (uint32_t j = 0; j < n; ++j) {
-                        const uint32_t c0 = key_tile(j) * kKeys;
-                        for (uint32_t c = c0; c < c0 + kKeys && c <= t; ++c) {
-                            if (!(seen(c) & 1u)) continue;
-                            const __half *col = a.v + ((uint64_t)hk * D + d0) * a.pitch + c;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const __half v = col[(uint64_t)i * a.pitch];
-                                if (!finite_bits(__half_as_ushort(v))) o[i] = __float_as_uint(__uint_as_float(o[i]) + __half2float(v));
-                            }
-                        }
-                    }
-                }
                 if (t < a.columns) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) dst[(uint64_t)(d0 + i) * step] = __float2half_rn(__uint_as_float(o[i]) * inv);
@@ -501,13 +518,32 @@ k44_window_attn_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     __syncthreads();
     ptx::tc_fence_after();
     if (warp == 1) ptx::tmem_dealloc(tmem, kTmemCols);
+    // Values that were kept from the tensor cores: a column that sees one gets it, on the canvas, where the output is by now. Here, because it
+    // hardly ever runs and took registers from the softmax (4 us of four prompts of 1000, 5 of 8192 tokens; here 1 and nothing).
+    if (*flagged == 0u || *abort_word != 0u || threadIdx.x >= 128u || t_first + threadIdx.x >= a.columns) return;
+    ptx::fence_proxy_async();
+    const Sight sight(a, t_first + threadIdx.x);
+#pragma unroll 1
+    for (uint32_t j = 0; j < n; ++j) {
+        const uint32_t kt = key_tile(j);
+        if (a.v_flags[hk * (a.pitch / 64u) + kt] == 0u) continue;
+        const uint32_t see0 = sight.seen(kt * kKeys), see1 = sight.seen(kt * kKeys + 32u);
+        const uint4 *marks = a.v_marks + ((uint64_t)hk * (a.pitch / 64u) + kt) * D;
+        __half *dst = a.out + (uint64_t)hq * D * a.pitch + sight.t;
+#pragma unroll 4
+        for (uint32_t d = 0; d < D; ++d, dst += a.pitch) {
+            const uint4 w = marks[d];
+            const bool up = ((w.x & see0) | (w.y & see1)) != 0u, down = ((w.z & see0) | (w.w & see1)) != 0u;
+            if (up || down) *dst = __float2half_rn(__half2float(*dst) + (up ? INFINITY : 0.f) + (down ? -INFINITY : 0.f));
+        }
+    }
 }
 
 }  // namespace
 
 uint64_t window_attn_scratch_bytes(uint32_t pitch, uint32_t h_kv, uint32_t head_dim) {
     const uint64_t row = (uint64_t)pitch * head_dim * 2u;
-    return 2u * kv8_align(h_kv * row) + kv8_align((uint64_t)h_kv * (pitch / 64u) * 4u);
+    return 2u * kv8_align(h_kv * row) + kv8_align((uint64_t)h_kv * (pitch / 64u) * 4u) + (uint64_t)h_kv * (pitch / 64u) * head_dim * sizeof(uint4);
 }
 
 void window_attn_place(WindowAttnArgs &a, void *scratch) {
@@ -515,7 +551,8 @@ void window_attn_place(WindowAttnArgs &a, void *scratch) {
     uint8_t *p = (uint8_t *)scratch;
     a.k_rows = (__half *)p; p += kv8_align(a.h_kv * row);
     a.v_rows = (__half *)p; p += kv8_align(a.h_kv * row);
-    a.v_flags = (uint32_t *)p;
+    a.v_flags = (uint32_t *)p; p += kv8_align((uint64_t)a.h_kv * (a.pitch / 64u) * 4u);
+    a.v_marks = (uint4 *)p;
 }
 
 cudaError_t window_attn_setup() {

@@ -193,3 +193,30 @@ def test_cached_keys_beyond_fp16_are_held_as_the_largest_number(dim):
         if part != "tail_block":
             assert np.array_equal(b[..., :6, :] if part == "k_tail" else b[..., :6] if part == "v_tail" else b[:, :, :1], a[part][..., :6, :] if part == "k_tail" else a[part][..., :6] if part == "v_tail" else a[part][:, :, :1], equal_nan=part != "codes"), part
     one.plan.close()
+
+
+# ---- values that are not finite ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim,columns,seq,window,sinks", [(64, 1000, 500, 0, 0), (128, 1000, 500, 0, 0), (64, 900, 900, 150, 70), (128, 333, 111, 0, 0), (64, 70, 70, 0, 0)])
+def test_values_that_are_not_finite_reach_the_columns_that_see_them(dim, columns, seq, window, sinks):
+    """One of a kind in some tiles, a whole tile of them, the first and last columns of tiles, hidden ones between seen ones."""
+    h_q, h_kv = 4, 2
+    rng = np.random.default_rng(columns + dim)
+    pitch, rq, rk = ops.pitch_of(columns), h_q * dim, h_kv * dim
+    body = rng.normal(0, 1, (rq + 2 * rk, pitch)).astype(np.float16)
+    v = body[rq + rk:]
+    for c in (0, 7, 8, 63, 64, 127, 300, 447, 448, 499, 500, 512, 640, 899):
+        if c < columns:
+            v[rng.integers(0, rk), c] = rng.choice([np.inf, -np.inf, np.nan])
+    v[rk - 1, 320: 384] = np.nan
+    v[3, columns - 1], v[3, columns - 2] = np.inf, -np.inf
+    v[:, columns:] = np.nan
+    plan, canvas = ops.make_plan(body, rq, columns)
+    plan.add_window_attn(0, rq * pitch, (rq + rk) * pitch, (rq + 2 * rk) * pitch, h_q, h_kv, dim, seq, window=window, sinks=sinks, theta=ops.THETA)
+    plan.execute()
+    assert plan.status() == 0
+    x = body[:, :columns].astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want, bound = D.window_attention(x[:rq], x[rq: rq + rk], x[rq + rk:], h_q, h_kv, seq, columns, window, sinks, ops.THETA)
+    assert not np.isfinite(want).all()
+    ops.within(ops.read(canvas, pitch)[rq + 2 * rk:, :columns], want, bound, "window attention")
+    plan.close()
