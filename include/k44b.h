@@ -187,9 +187,10 @@ int k44b_plan_set_sequences(void *plan, const int32_t *h_cache_columns, const in
  * (set_positions: the first n columns, -1 = idle, the initial state of all; an advancing arg-max moves the positions of the columns
  * that are not idle on by one). q and k are rotated at that position and stay as they are on the canvas, k and v are appended, and
  * the column attends to positions 0 .. position under the same window and sinks as above. An idle column gets zeros and its cache is
- * left alone. h_q / h_kv up to 16, at most 4096 columns. A position may go back: the positions behind it are given up, and those of its
- * block keep their 8-bit values where the block was complete. A position outside the cache leaves its column idle and sets status
- * bit 4. One execution of a plan at a time, and one plan at a time on a cache. */
+ * left alone. h_q / h_kv up to 16, at most 4096 columns. A position may go back: the positions behind it are given up, and those before
+ * it in its block keep the values that the cache holds: the FP16 rows as long as tail_block names that block, which it does from the
+ * block's first token here until a token of another block comes (or a prompt is filled in), and the 8-bit values otherwise. A position
+ * outside the cache leaves its column idle and sets status bit 4. One execution of a plan at a time, and one plan at a time on a cache. */
 int k44b_plan_add_kv8_attn(void *plan, const char *name, const k44b_kv8_cache *cache, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off,
                            uint32_t h_q, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling);
 int k44b_plan_set_positions(void *plan, const int32_t *h_positions, uint32_t n, void *stream);

@@ -162,3 +162,69 @@ def test_a_sequence_behind_the_last_column_is_refused():
     assert plan.status() == 0
     assert cache.views()["tail_block"].flatten().tolist() == [0, 0, -1, 0]
     plan.close()
+
+
+def fill_and_step(n, filled, dim, llama3=False, back=None):
+    """The first `filled` of n tokens from a prompt, the others one by one, then one at position `back`; the cache's arrays."""
+    import torch
+    h_kv = 2
+    rk = h_kv * dim
+    data = np.random.default_rng(31).normal(0, 1, (2 * rk, 256)).astype(np.float16)
+    cache = KV8Cache(1, h_kv, dim, 256)
+    if filled:
+        pitch = ops.pitch_of(filled)
+        body = np.zeros((2 * rk, pitch), dtype=np.float16)
+        body[:, :filled] = data[:, :filled]
+        plan, _ = ops.make_plan(body, 0, filled)
+        plan.add_kv8_fill(cache, 0, rk * pitch, filled, theta=ops.THETA, llama3=llama3)
+        plan.set_sequences([0], [filled])
+        plan.execute()
+        assert plan.status() == 0
+        plan.close()
+    body = np.ones((3 * rk, 64), dtype=np.float16)
+    plan, canvas = ops.make_plan(body, rk, 1)
+    plan.add_kv8_attn(cache, 0, rk * 64, 2 * rk * 64, 3 * rk * 64, h_kv, theta=ops.THETA, llama3=llama3)
+    steps = [(t, t) for t in range(filled, n)] + ([] if back is None else [(back, 255)])
+    for t, token in steps:
+        canvas.view(-1, 64)[rk: 3 * rk, 0] = torch.from_numpy(data[:, token].copy()).cuda()
+        plan.set_positions([t])
+        plan.execute()
+    assert plan.status() == 0
+    out = ops.read(canvas, 64)[3 * rk:, 0].copy()
+    plan.close()
+    return ops.cache_arrays(cache), out
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("llama3", [False, True])
+def test_a_prompt_and_tokens_leave_the_same_bits(dim, llama3):
+    n = 150
+    want, out = fill_and_step(n, 0, dim, llama3)
+    rest = n % 64
+    for filled in (149, 128, 100, 64, 63, 1):
+        got, o = fill_and_step(n, filled, dim, llama3)
+        assert np.array_equal(got["codes"][:, :, :2], want["codes"][:, :, :2]) and np.array_equal(got["scales"][:, :, :2], want["scales"][:, :, :2])
+        assert np.array_equal(got["k_tail"][:, :, :rest], want["k_tail"][:, :, :rest]) and np.array_equal(got["v_tail"][..., :rest], want["v_tail"][..., :rest])
+        assert np.array_equal(got["tail_block"], want["tail_block"]) and np.array_equal(o, out)
+    # and they are the keys at their positions
+    k = np.random.default_rng(31).normal(0, 1, (4 * dim, 256)).astype(np.float16)[:dim, 128:n].astype(np.float64).T
+    k = D.rotated(k, np.arange(128, n), ops.THETA, llama3)
+    assert np.all(np.abs(want["k_tail"][0, 0, :rest] - k) <= D.HALF16 * np.abs(k) + 2.0 ** -22 * np.abs(k).max() + D.TINY16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_going_back_into_a_block_that_has_just_been_completed(dim):
+    """Its FP16 rows are still there until a token of another block comes; after that, or where a prompt filled it, it starts from its 8 bits."""
+    back = 40
+    kept, _ = fill_and_step(128, 0, dim)
+    rows, out_rows = fill_and_step(128, 0, dim, back=64 + back)
+    assert np.array_equal(rows["k_tail"][:, :, :back], kept["k_tail"][:, :, :back]) and np.array_equal(rows["v_tail"][..., :back], kept["v_tail"][..., :back])
+    filled, out_filled = fill_and_step(128, 128, dim, back=64 + back)
+    for h in range(2):
+        k, v = ops.block_values(kept, 0, h, 1, dim)
+        assert np.array_equal(filled["k_tail"][0, h, :back], k[:back].astype(np.float32).astype(np.float16))
+        assert np.array_equal(filled["v_tail"][0, h, :, :back].T, v[:back].astype(np.float32).astype(np.float16))
+    assert np.array_equal(filled["k_tail"][:, :, back], rows["k_tail"][:, :, back]) and (rows["tail_block"] == 1).all() and (filled["tail_block"] == 1).all()
+    later, out_later = fill_and_step(129, 0, dim, back=64 + back)
+    assert np.array_equal(later["k_tail"][:, :, :back], filled["k_tail"][:, :, :back]) and np.array_equal(later["v_tail"][..., :back], filled["v_tail"][..., :back])
+    assert np.array_equal(out_later, out_filled) and np.isfinite(out_rows).all()
