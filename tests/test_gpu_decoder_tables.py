@@ -164,6 +164,39 @@ def test_a_sequence_behind_the_last_column_is_refused():
     plan.close()
 
 
+@pytest.mark.parametrize("stay", [False, True])
+def test_positions_that_an_advancing_arg_max_moves_to_the_end(stay):
+    """Without a limit a column runs out of the cache: it is idle then, its cache is left alone and the status says so; with one it stays
+    at the last position. The other columns go on."""
+    import torch
+    h_q, h_kv, dim, max_seq = 2, 1, 64, 100
+    positions = np.array([max_seq - 1, 5, -1, 62], dtype=np.int32)
+    d = ops.Decoder(h_q, h_kv, dim, positions.size, max_seq, seed=21)
+    d.history()
+    d.cache.views()["tail_block"].copy_(torch.tensor([[1], [0], [-1], [0]], dtype=torch.int32))
+    body = d.rng.normal(0, 1, (d.rq + 2 * d.rk, d.pitch)).astype(np.float16)
+    d.canvas[: body.size] = torch.from_numpy(body.reshape(-1)).cuda()
+    d.plan.add_argmax(0, d.rq, advance=True, max_seq=max_seq if stay else 0)
+    d.plan.set_positions(positions)
+    for step in range(3):
+        before = ops.cache_arrays(d.cache)
+        d.canvas[body.size:] = float(ops.SENTINEL)
+        d.plan.execute_graph() if step else d.plan.execute()
+        now = positions.copy()
+        if step and stay:
+            now[0] = max_seq - 1
+        elif step:
+            now[0] = -1                                                # what the kernels make of max_seq and beyond
+        if stay or step == 0:
+            assert d.plan.status() == 0
+        else:
+            with pytest.raises(NativeError, match="status 0x10:"):
+                d.plan.status()
+        d.check(now, body, ops.read(d.canvas, d.pitch)[body.shape[0]:, : d.columns], before, ops.cache_arrays(d.cache))
+        positions[positions >= 0] += 1
+    d.plan.close()
+
+
 def fill_and_step(n, filled, dim, llama3=False, back=None):
     """The first `filled` of n tokens from a prompt, the others one by one, then one at position `back`; the cache's arrays."""
     import torch
