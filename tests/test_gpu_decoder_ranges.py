@@ -220,3 +220,36 @@ def test_values_that_are_not_finite_reach_the_columns_that_see_them(dim, columns
     assert not np.isfinite(want).all()
     ops.within(ops.read(canvas, pitch)[rq + 2 * rk:, :columns], want, bound, "window attention")
     plan.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_odd_keys_and_values_from_a_prompt_and_token_by_token(dim):
+    """Infinities, NaN and numbers at the end of FP16 in complete blocks and in the open one leave the same codes, scales and rows (the code
+    of a NaN may have either sign)."""
+    import torch
+    h_kv, n, pitch = 3, 200, 256
+    rk = h_kv * dim
+    rng = np.random.default_rng(dim)
+    body = rng.normal(0, 1, (2 * rk, pitch)).astype(np.float16)
+    for x in (np.nan, np.inf, -np.inf, 65504, -60000):
+        for _ in range(6):
+            body[rng.integers(0, 2 * rk), rng.integers(0, n)] = x
+    prompt = ops.KV8Cache(1, h_kv, dim, 256)
+    plan, _ = ops.make_plan(body, 0, n)
+    plan.add_kv8_fill(prompt, 0, rk * pitch, n, theta=ops.THETA)
+    plan.set_sequences([0], [n])
+    plan.execute()
+    assert plan.status() == 0
+    plan.close()
+    one = ops.Decoder(h_kv, h_kv, dim, 1, 256)
+    for t in range(n):
+        x = np.zeros((3 * rk, one.pitch), dtype=np.float16)
+        x[rk:, 0] = body[:, t]
+        one.step([t], tag=False, check=False, body=x)
+    a, b = ops.cache_arrays(prompt), ops.cache_arrays(one.cache)
+    r, whole = n % 64, n // 64
+    nan = (a["codes"][:, :, :whole] & 127) == 127
+    assert nan.any() and np.array_equal(nan, (b["codes"][:, :, :whole] & 127) == 127)
+    assert np.array_equal(a["codes"][:, :, :whole][~nan], b["codes"][:, :, :whole][~nan]) and np.array_equal(a["scales"][:, :, :whole], b["scales"][:, :, :whole])
+    assert np.array_equal(a["k_tail"][:, :, :r], b["k_tail"][:, :, :r], equal_nan=True) and np.array_equal(a["v_tail"][..., :r], b["v_tail"][..., :r], equal_nan=True)
+    one.plan.close()
