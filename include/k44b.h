@@ -155,7 +155,8 @@ int k44b_plan_get_next_tokens(void *plan, int32_t *h_tokens, uint32_t n, void *s
  * Prompt attention with a sliding window and sinks: like add_rope_attn (blocks of seq_len columns, grouped-query heads, head_dim 64
  * or 128), but seq_len may be any length, and column t of a sequence that starts at s0 sees column c if s0 <= c <= t and (window == 0,
  * or c > t - window, or c < s0 + sinks). q and k are rotated on the way and stay as they are on the canvas; out must not overlap
- * them. Prompts of different lengths are padded behind their last token. A hidden column does not count, whatever it holds. */
+ * them. Prompts of different lengths are padded behind their last token. A hidden column does not count, whatever it holds; a
+ * value that is not finite reaches every column that sees it, whatever its weight. */
 int k44b_plan_add_window_attn(void *plan, const char *name, uint64_t q_off, uint64_t k_off, uint64_t v_off, uint64_t out_off, uint32_t h_q,
                               uint32_t h_kv, uint32_t head_dim, uint32_t seq_len, uint32_t window, uint32_t sinks, float rope_theta, int llama3_scaling);
 /* Key / value cache of 8 bits. It lives in device memory of the caller (so that a prompt plan can fill it and a decode plan read it)

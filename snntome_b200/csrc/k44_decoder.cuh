@@ -65,7 +65,7 @@ struct Kv8AttnArgs {
     uint32_t *status = nullptr;
     uint4 *q_frag = nullptr;                         // [column][head]: the group's rotated q as operand words
     float *partial = nullptr;                        // [worker][2][8 or 16 heads][head_dim + 2]
-    uint32_t *counters = nullptr;                    // [column][head], zero between launches
+    uint32_t *counters = nullptr;                    // [column][head]: units of it that have arrived; every run clears them first
     uint32_t pitch = 0, columns = 0, h_q = 0, window = 0, sinks = 0;
     uint32_t workers = 0, spread = 1;                // warps, and their step over the shares (set by the launcher)
     unsigned long long wait_cycles = 0;
@@ -102,7 +102,7 @@ struct LogprobArgs {
     const int *targets = nullptr;
     float *logprobs = nullptr, *entropy = nullptr, *top_logprobs = nullptr;
     int *top_rows = nullptr;
-    float4 *parts = nullptr;                         // [column][chunk]: maximum, sum of e^(x - max), sum of e^(x - max) (x - max)
+    float4 *parts = nullptr;                         // [column][chunk]: M, L and W of k44_logprobs.cu, in powers of 2
     uint16_t *group_max = nullptr;                   // [column][group]: order of the largest value of 64 rows
     uint32_t *status = nullptr;
     unsigned long long wait_cycles = 0;

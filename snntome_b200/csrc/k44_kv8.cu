@@ -2,7 +2,8 @@
 //
 // Format (k44_decoder.cuh): blocks of 64 tokens of one column and head, e4m3 codes with one FP32 scale per block for keys and
 // one for values,  scale = max(amax, 2^-24) / 448,  code = e4m3(x / scale);  infinities count as the largest FP16 number, a NaN
-// stays a NaN of its own value; keys are rotated, and rounded to FP16, where finite ones end at the largest number. The open block is kept as FP16 rows, so that a scale is chosen once, with all 64 tokens known.
+// stays a NaN of its own value; keys are rotated, and rounded to FP16, where finite ones end at the largest number. The open block is kept
+// as FP16 rows, so that a scale is chosen once, with all 64 tokens known.
 // A block is brought to 8 bits by the step that appends its last token and read in 8 bits from the next block on.
 #include "k44_decoder.cuh"
 #include "k44_ptx.cuh"
@@ -75,14 +76,15 @@ __device__ __forceinline__ uint32_t pack2_finite(float a, float b) {
 
 // ---- filling the cache from a prompt ----------------------------------------------------------------------------------------
 // CTA = the keys or the values of one block of 64 tokens of one sequence, some of its heads one after the other. Keys are rotated and
-// rounded to FP16 first, then treated as the step by step path treats them. HBM-bound: 4 bytes read and 2 written per pair of key and
-// value elements. Keys pass through shared memory once, to be turned from channel rows to token rows: a thread owns one token and 8
+// rounded to FP16 first, then treated as the step by step path treats them. What it cannot do without is HBM: 4 bytes read and 2 written
+// per pair of key and value elements. Keys pass through shared memory once, to be turned from channel rows to token rows: a thread owns one token and 8
 // rotation pairs, neighbours the next pairs, so that table and codes are read and written in whole sectors and a token's elements stay
 // in registers from the rotation to the code. Values need no turning: a thread takes 8 tokens of a channel from the canvas to their
 // codes. The next head's rows load meanwhile. Columns are read from the 16-byte boundary below a sequence's first one.
 // 64 prompts of up to 512 tokens, 8 heads of 64: 17.5 us for 50 MB. Keys and values in one CTA 20.7 (123 registers, half as many
 // CTAs); without heads in a row 25 (each CTA waits for its length, rows and angles in turn), with 2 or 3 18 to 19, with 8 20 (too
-// few CTAs). What is left is those waits of the first CTAs and the last ones' uneven end; HBM is at a fifth while it runs.
+// few CTAs). With 128 dimensions 32.8 for 100 MB. What bounds it is those waits of the first CTAs, CTAs of the grid that a short sequence
+// leaves without work, and the last ones' uneven end; HBM is at a fifth while it runs.
 template <int D>
 __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(const Kv8FillArgs a, uint32_t heads) {
     dep_enter();
@@ -276,13 +278,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 4 : 2) k44_kv8_fill_kernel(cons
 // p' / number), while the accumulator is kept in units of 2^e and moves by a power of two, exactly, where a block has another e: what is
 // rounded to FP16 is a weight relative to the largest one, not to that times its block's scale, or one loud block (a value of
 // 6e4 next to values of 1) would leave nothing of the weights behind it. p' <= 1 is held as 2^15 p', so that FP16 has whole
-// precision down to 2^-29 and something down to 2^-40 of the largest weight.
+// precision down to 2^-29 and something down to 2^-40 of the largest weight. The rounding is the tensor cores' type, 2^-11 of a weight, of
+// the order of the output's own (2.4e-4 relative to 64 bits; with weights in 32 bits 2.0e-4).
 // Half of q (a rotated pair of FP16 numbers may be sqrt(2) longer than the largest one) is split into two FP16 numbers (high and low
 // part): with exact codes the scores are then as good as in 32 bits. With up to 8 heads the low parts are rows 8 to 15 of the operand,
 // which would be empty, and cost nothing.
-// Measured, both launches: 48 columns at up to 8190 positions, 32 heads on 8 of 128 dimensions: 78 to 80 us for 348 MB (4.4 TB/s; the
-// same without the products: what bounds it is bytes in flight and the last warps' end); 64 columns at 511, D = 64, each
-// completing a block: 24 us; 64 columns at up to 16000 with a window of 1024: 28; one column at 1500: 15, a chain of latencies.
+// Measured, both launches: 48 columns at up to 8190 positions, 32 heads on 8 of 128 dimensions: 79 us for the 350 to 400 MB
+// of the lengths drawn (4.4 to 4.9 TB/s; the same without the products; 192 KB in flight per SM are 4 us of HBM's full rate, so what is
+// lost is the start and the last warps' uneven end); 64 columns at 511, D = 64, each completing a block: 24 us; 64 columns at up to 16000 with a
+// window of 1024: 28; one column at 1500: 15, a chain of latencies. 16 query heads on one: 27 us for 64 columns at 511 (32 heads on 2 of
+// 64), 95 for 48 columns at up to 8190 (32 on 2 of 128, 82 MB): few (column, head) pairs, long chains of products in each warp.
 constexpr float kWeightBits = 15.f;
 constexpr uint32_t kOpenWeight = 4;                              // an open block: one and a half times the bytes, and the work around it
 // warps per SM and granules per warp (192 KB of an SM's shared memory in all): as many warps as the registers allow
@@ -928,6 +933,7 @@ cudaError_t launch_kv8_fill(const Kv8FillArgs &a, bool pdl, cudaStream_t s) {
     // no sequence is longer than any of these
     const uint32_t longest = std::min(a.seq_len, std::min(a.columns, a.cache.max_seq)), H = a.cache.h_kv;
     const uint32_t blocks = (longest + kKv8Block - 1u) / kKv8Block, seqs = (a.columns - 1u) / a.seq_len + 1u;
+    // as many heads in a row as leave eight CTAs for each of 148 SMs, up to four
     const uint32_t heads = (uint32_t)std::max<uint64_t>(1u, std::min<uint64_t>(4u, 2ull * blocks * seqs * H / 1184u));
     const dim3 grid(blocks, 2u * ((H + heads - 1u) / heads), seqs);
     return a.cache.head_dim == 64u ? launch_dep(k44_kv8_fill_kernel<64>, grid, dim3(256), 0, pdl, s, a, heads)

@@ -22,7 +22,7 @@ __device__ __forceinline__ bool finite_bits(uint32_t h) { return (h & 0x7c00u) !
 // ---- operands ---------------------------------------------------------------------------------------------------------------
 // CTA = 64 columns of a few heads of k, or of one head of v. Columns behind the plan's last one become zero. Values of v that are
 // not finite become zero too, and their tile is flagged: a hidden column has weight 0, but 0 * inf is not 0, so such values must not reach the
-// tensor cores; the attention adds them to the columns that do see them. A flagged tile leaves a word of 64 bits per dimension for the
+// tensor cores; the attention adds them to the columns that do see them, whatever their weight. A flagged tile leaves a word of 64 bits per dimension for the
 // columns that hold +inf (or NaN) and one for -inf (or NaN): a column of the output needs an AND with what it sees, not the values
 // (2048 columns, 8 heads on 2 of 64, one infinity for all to see: 47 us without, 1867 with the values read, 61 with the words). The rotated q and k, and the weights, are rounded to FP16, the
 // tensor cores' type: 2^-11 of each, so some 4e-4 of the output's size, of the order of its own rounding to FP16. q and k are held at
@@ -144,13 +144,15 @@ __global__ void __launch_bounds__(256) k44_window_operands_kernel(const WindowAt
 // Warp 0 copies (TMA), one thread of warp 1 issues the MMAs, warps 2-5 are the softmax: a thread owns one column (= TMEM lane).
 // Tensor memory: a buffer of 64 columns of scores, over whose first half the weights are written as FP16 pairs once the scores are
 // read (the A operand of the second product), and D columns of output. 128 x 64 exponentials take 512 cycles of the SM's 16 per
-// cycle, their products 128 (D = 64) or 256. Nothing of it overlaps within one column's chain (scores, maximum, weights, output), so
+// cycle, the two products of a tile 256 (D = 64) or 512 at 4096 multiplications a cycle: at D = 128 the tensor cores have as much to do
+// as the exponential unit (28 and 25 % busy), at D = 64 half as much (25 and 45 %). Nothing of it overlaps within one column's chain (scores, maximum, weights, output), so
 // what counts is how many chains an SM holds: D = 64 runs four CTAs per SM (128 columns of tensor memory each, 80 registers, the
 // second half of the scores read twice, one stage of keys and values), D = 128 two, each with a second buffer in which the next
-// scores are made meanwhile. Both launches, 8192 tokens, 32 heads on 8, window 1024, D = 64: 154 us (with two stages 160, three CTAs
-// of more registers 172, two CTAs with two buffers 164, two warps to a row 180); four prompts of 1000, 32 heads on 8, D = 128: 85 us
-// (with one buffer 107). Without its exponentials the former still takes 142, without exponentials and products 128: the chain's
-// waits and reads of tensor memory bound it.
+// scores are made meanwhile. Both launches, 8192 tokens, 32 heads on 8, window 1024, D = 64: 154 to 157 us (with two stages 160, three CTAs
+// of more registers 172, two CTAs with two buffers 164, two warps to a row 180); four prompts of 1000, 32 heads on 8, D = 128: 87 us
+// (with one buffer 107). Without its exponentials the former still takes 142, without exponentials and products 128: in this kernel the
+// chain's waits and reads of tensor memory bound it. Scores four times as large as these unit normal queries and keys give, whose maxima
+// keep growing, take 179 and 119 us: the output is read and written back at every rescale.
 // The output is rescaled only when a column's maximum has grown by more than 2^8 since the last time: weights up to 256 are as
 // exact in FP16 as weights up to 1, and the sum is kept against the same maximum. Weights are held times 2^7 (up to 2^15), so that FP16
 // has whole precision down to 2^-21 and something down to 2^-32 of the maximum: thousands of keys far below a first one still add up.
@@ -174,7 +176,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two at a time: (a.x * b + c, a.y * b + c), and sums
+// the largest of three
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -566,7 +568,7 @@ cudaError_t launch_window_attn(const WindowAttnArgs &a, const WindowAttnMaps &m,
     const uint32_t tiles = (a.columns + 127u) / 128u;
     const uint32_t wide = std::min(2u * tiles, a.pitch / 64u), turned = a.h_kv;
     // several heads per CTA (they share the angles, and one head's rows load while another's are turned) where that leaves CTAs enough:
-    // 8192 tokens, 32 heads on 32: 175 us for both launches, with one head per CTA 180
+    // 8192 tokens, 32 heads on 32: 175 us for both launches, with one head per CTA 180. Enough: four for each of 148 SMs.
     const uint32_t heads = std::max(1u, std::min(8u, wide * turned / 592u));
     const dim3 g1(wide, (turned + heads - 1u) / heads + a.h_kv), g2(a.h_q, tiles);
     cudaError_t e;
