@@ -544,11 +544,12 @@ __global__ void __launch_bounds__(kWarps<D, WIDE> * 32, 1) k44_kv8_attn_kernel(c
         if (at.pos >= 0 && unit + 1u < at.seen.units) {
             const float2 sc = __ldg(a.cache.scales + ((uint64_t)at.col * H + at.head) * a.cache.blocks + block_of(at.seen, unit));
             // The cache's own scales lie between 2^-33 and 2^8. Larger ones are left for the number, whose range is that of 32 bits; one below
-            // 2^-60, such as the 0 of a block that nobody has written, counts as that: its values come out below 2^-51.
-            const float scale = sc.y < pow2(-60) ? pow2(-60) : sc.y;
+            // 2^-60, such as the 0 of a block that nobody has written, counts as that: its values come out below 2^-51, and a hidden score
+            // of -inf times a key's scale stays -inf.
+            const float key = sc.x < pow2(-60) ? pow2(-60) : sc.x, scale = sc.y < pow2(-60) ? pow2(-60) : sc.y;
             sc_exp = min(60, (int)(__float_as_uint(scale) >> 23 & 255u) - 127);
             const float number = scale * pow2(-sc_exp);
-            sc_mul = sc.x * sm; sc_log = log2f(number); sc_inv = 1.0f / number;
+            sc_mul = key * sm; sc_log = log2f(number); sc_inv = 1.0f / number;
         }
     };
     auto fetch_head = [&]() {

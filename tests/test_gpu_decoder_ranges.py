@@ -23,7 +23,7 @@ def test_a_loud_block_leaves_the_weights_of_the_others(h_q, h_kv, dim, columns):
     scale, are as small as 2^-28 of that block's; a warp's share is some 17 blocks, which hold several of both kinds. Magnitudes of the
     other blocks differ by up to 10^4."""
     import torch
-    blocks = 30720 // (columns * h_kv)
+    blocks = 30000 // (columns * h_kv)
     pos = blocks * 64 + 20
     d = ops.Decoder(h_q, h_kv, dim, columns, pos + 5, seed=41)
     g = torch.Generator(device="cuda").manual_seed(42)
@@ -67,6 +67,14 @@ def test_blocks_of_a_cleared_cache_are_zeros(h_q, dim):
     d = ops.Decoder(h_q, 1, dim, 3, 300, seed=9)
     d.step([130, 64, 299])
     d.step([131, 65, 5])
+    d.plan.close()
+
+
+@pytest.mark.parametrize("h_q,dim", [(4, 64), (16, 128)])
+def test_blocks_of_a_cleared_cache_at_the_edges_of_a_window(h_q, dim):
+    d = ops.Decoder(h_q, 1, dim, 3, 300, 60, 100, seed=10)
+    d.step([216, 130, 299])
+    d.step([217, 131, 110])
     d.plan.close()
 
 
